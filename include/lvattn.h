@@ -95,6 +95,39 @@ int lv_store_latents(const void* latent, int64_t latent_stride_t, int32_t num_to
                      const int32_t* slot_mapping, int32_t elem_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------
+ * Rotary positions on queries and keys, optionally after an RMS norm of each head. No counterpart in the reference's
+ * attention interface, which takes queries and keys as they leave this (lean_vllm/attention/abstract.py:107-146).
+ *
+ * q: [T, Hq, D], k: [T, Hkv, D] with their own token and head strides and unit dim stride; num_heads or num_kv_heads may
+ * be 0. positions[T]: int64. table: fp32 [max_position, rotary_dim], contiguous: the cosines of rotary_dim / 2 pairs,
+ * then their sines. Pair i is dims (i, i + rotary_dim / 2) or, with interleaved != 0, (2 i, 2 i + 1):
+ *   y_a = x_a cos - x_b sin, y_b = x_b cos + x_a sin; dims from rotary_dim on are copied.
+ * q_weight / k_weight (either may be NULL: not normed): [D] of the same dtype, contiguous; x is first
+ *   x * rsqrt(mean(x^2) + eps) * weight.
+ * Computed in fp32, rounded once. q_out, k_out: same shapes, own strides; each may be its input (the same pointer and
+ * strides), and must not overlap it otherwise. A negative position (a captured step's padding row) rotates as position 0; one at or
+ * past max_position gives NaN in the rotated dims. */
+int lv_rotary(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+              int64_t k_stride_h, const int64_t* positions, const float* table, int64_t max_position,
+              int32_t rotary_dim, int32_t interleaved, const void* q_weight, const void* k_weight, float eps,
+              int32_t num_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, void* q_out,
+              int64_t q_out_stride_t, int64_t q_out_stride_h, void* k_out, int64_t k_out_stride_t,
+              int64_t k_out_stride_h, int32_t dtype, void* stream);
+
+/* lv_rotary on the way into the paged cache: the queries to q_out, the rotated keys and the values (v: [T, Hkv, D], own
+ * strides, copied as they are) to the caches by slot, as lv_store_kvcache stores them (slot -1: nothing stored; its query
+ * is rotated all the same). Two tokens of one slot: either may stay. num_heads may be 0 (a step that only fills the
+ * cache). */
+int lv_append_kvcache(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                      int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                      const int64_t* positions, const float* table, int64_t max_position, int32_t rotary_dim,
+                      int32_t interleaved, const void* q_weight, const void* k_weight, float eps, int32_t num_tokens,
+                      int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, void* q_out, int64_t q_out_stride_t,
+                      int64_t q_out_stride_h, void* k_cache, void* v_cache, int64_t cache_stride_block,
+                      int64_t cache_stride_token, int64_t cache_stride_head, int32_t block_size,
+                      const int32_t* slot_mapping, int32_t dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
  * Paged attention over a step: pure decode, chunked prefill, or a mixed batch in one kernel.
  * Replaces AttentionBackend.decode / prefill / forward for this backend (lean_vllm/attention/abstract.py:118-176;
  * math of TorchAttention.decode/prefill, lean_vllm/attention/torch_backend.py:62-103).

@@ -25,6 +25,13 @@ _PROTOTYPES = {
     "lv_store_kvcache": (ctypes.c_int, [_P, _P, c_int64, c_int64, c_int32, c_int32, c_int32, _P, _P,
                                         c_int64, c_int64, c_int64, c_int32, _P, c_int32, _P]),
     "lv_store_latents": (ctypes.c_int, [_P, c_int64, c_int32, c_int32, _P, _P, c_int32, _P]),
+    "lv_rotary": (ctypes.c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, _P, c_int64, c_int32, c_int32, _P, _P,
+                                 c_float, c_int32, c_int32, c_int32, c_int32, _P, c_int64, c_int64, _P, c_int64,
+                                 c_int64, c_int32, _P]),
+    "lv_append_kvcache": (ctypes.c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, _P,
+                                         c_int64, c_int32, c_int32, _P, _P, c_float, c_int32, c_int32, c_int32,
+                                         c_int32, _P, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int32,
+                                         _P, c_int32, _P]),
     "lv_paged_attention_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
                                                       c_int32]),
     "lv_paged_attention": (ctypes.c_int, [_P, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int32, _P,
@@ -123,6 +130,15 @@ def call(name: str, *args):
         msg = load().lv_last_error().decode(errors="replace")
         raise LvError(f"{name}: {msg} (status {rc})")
     return rc
+
+
+def call_on(device: torch.device, name: str, *args):
+    """``call`` on ``device``'s current stream (the C function's last argument), with ``device`` current: a launch and
+    the library's per-device state go by the current device, which the tensors' need not be."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return call(name, *args, stream_of(device))
+    with torch.cuda.device(device):
+        return call(name, *args, stream_of(device))
 
 
 def query(name: str, *args):

@@ -79,6 +79,15 @@ def check_key_lengths(lens: torch.Tensor, block_tables: torch.Tensor, block_size
                          f" is -1")
 
 
+def check_positions(positions: torch.Tensor, max_position: int) -> None:
+    """Every position has a row in the rotary table (a padding row's negative one takes row 0)."""
+    p = _host(positions).reshape(-1)
+    bad = p >= max_position
+    if bad.any():
+        i = _first(bad)
+        raise ValueError(f"positions[{i}] = {int(p[i])} is past a table of {max_position} positions")
+
+
 def check_query_rows(cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor, num_tokens: int) -> None:
     """``cu_seqlens_q/k`` start at 0 and never fall, ``cu_seqlens_q`` ends at the token count, and no row has more
     queries than keys."""

@@ -1,0 +1,162 @@
+"""Rotary positions of queries and keys, after an RMS norm of each head where a model has one, on the GPU.
+
+What a layer does between its q/k/v projection and ``store_kvcache`` / ``forward``, in one launch (``lv_rotary``):
+``norm_rotary`` norms and rotates, ``apply_rotary`` only rotates; ``MI355XAttention.append_kvcache`` does either on the
+way into the paged cache. ``Packer.pack`` returns the ``positions`` they read. ``rotary_table`` lays out the cosines and
+sines once, for the plain frequencies or ones scaled to contexts longer than the trained ones.
+"""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import torch
+
+from . import _capi, checks
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None) -> tuple[np.ndarray, float]:
+    """Angle per position of each of the ``rotary_dim / 2`` pairs (float64), and the factor on cosines and sines.
+
+    ``scaling`` (None: ``base ** (-2 i / rotary_dim)``) names a ``rope_type``, as checkpoints' configurations do:
+
+    - ``linear``: positions divided by ``factor``;
+    - ``ntk``: the base raised by ``factor ** (r / (r - 2))``, so that the slowest pair is slowed by ``factor``;
+    - ``llama3``: pairs of fewer than ``low_freq_factor`` (1) turns over ``original_max_position_embeddings`` slowed by
+      ``factor``, of more than ``high_freq_factor`` (4) kept, a linear blend between;
+    - ``yarn`` (Peng et al., "YaRN", 2023): the blend linear over the pairs' indices, from ``beta_fast`` (32) turns to
+      ``beta_slow`` (1), and cosines and sines times ``attention_factor`` (``0.1 ln(factor) + 1``).
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_frequencies: the rotary width {rotary_dim} is not a positive even number")
+    if not base > 1:
+        raise ValueError(f"rotary_frequencies: base {base} is not above 1")
+    r, s = rotary_dim, dict(scaling or {})
+    kind = s.pop("rope_type", None) or s.pop("type", None) or "default"
+    exponents = np.arange(0, r, 2, dtype=np.float64) / r
+    inv = float(base) ** -exponents
+    if kind == "default":
+        return inv, 1.0
+    if kind not in ("linear", "ntk", "llama3", "yarn"):
+        raise ValueError(f"rotary_frequencies: rope_type {kind!r} is not one of default, linear, ntk, llama3, yarn")
+    factor = float(s.get("factor", 0.0))
+    if not factor >= 1.0:
+        raise ValueError(f"rotary_frequencies: rope_type {kind!r} needs a factor of at least 1, got {s.get('factor')}")
+    if kind == "linear":
+        return inv / factor, 1.0
+    if kind == "ntk":
+        if r == 2:
+            raise ValueError("rotary_frequencies: ntk scaling needs a rotary width above 2")
+        return (float(base) * factor ** (r / (r - 2))) ** -exponents, 1.0
+    trained = s.get("original_max_position_embeddings")
+    if not trained or trained <= 0:
+        raise ValueError(f"rotary_frequencies: rope_type {kind!r} needs original_max_position_embeddings")
+    if kind == "llama3":
+        low, high = float(s.get("low_freq_factor", 1.0)), float(s.get("high_freq_factor", 4.0))
+        if not 0 < low < high:
+            raise ValueError(f"rotary_frequencies: low_freq_factor {low} and high_freq_factor {high}")
+        kept = np.clip((trained * inv / (2 * math.pi) - low) / (high - low), 0.0, 1.0)
+        return inv * (kept + (1.0 - kept) / factor), 1.0
+
+    def pair_of(turns: float) -> float:  # twice the index of the pair that makes so many turns over the trained length
+        return r * math.log(trained / (2 * math.pi * turns)) / (2 * math.log(base))
+
+    fast, slow = float(s.get("beta_fast") or 32.0), float(s.get("beta_slow") or 1.0)
+    if not 0 < slow < fast:
+        raise ValueError(f"rotary_frequencies: beta_fast {fast} and beta_slow {slow}")
+    lo, hi = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), r - 1)
+    slowed = np.clip((np.arange(r // 2) - lo) / max(hi - lo, 1e-3), 0.0, 1.0)
+    amp = s.get("attention_factor")
+    return inv * (1.0 - slowed + slowed / factor), float(amp) if amp is not None else 0.1 * math.log(factor) + 1.0
+
+
+def rotary_table(rotary_dim: int, max_position: int, base: float = 10000.0, scaling: dict | None = None,
+                 device="cuda") -> torch.Tensor:
+    """fp32 ``[max_position, rotary_dim]``: each position's ``rotary_dim / 2`` cosines, then its sines. Angles are taken
+    in 64 bits (an fp32 angle at position 10^5 is off by up to 4e-3) and only the table is rounded."""
+    if max_position < 1:
+        raise ValueError(f"rotary_table: {max_position} positions")
+    inv, amp = rotary_frequencies(rotary_dim, base, scaling)
+    inv = torch.from_numpy(inv).to(device)
+    table = torch.empty(max_position, rotary_dim, dtype=torch.float32, device=device)
+    half, step = rotary_dim // 2, 1 << 16
+    for at in range(0, max_position, step):  # the 64-bit angles of 65536 positions at a time
+        angles = torch.arange(at, min(at + step, max_position), dtype=torch.float64, device=device)[:, None] * inv
+        table[at:at + step, :half] = angles.cos().mul_(amp)
+        table[at:at + step, half:] = angles.sin_().mul_(amp)
+    return table
+
+
+def check_rotary(what: str, heads: dict, positions, table, weights: dict) -> None:
+    """Raises ``ValueError`` unless every tensor of ``heads`` (name -> ``[T, H, D]`` or None) has the same T, D, dtype and
+    unit dim stride, ``positions`` is int64 ``[T]``, ``table`` fp32 ``[P, r]`` with r even and at most D, the ``weights``
+    ``[D]`` of the heads' dtype, and all are on one GPU."""
+    first = next((t for t in heads.values() if t is not None), None)
+    if first is None:
+        raise ValueError(f"{what}: no heads to rotate")
+    if first.dim() != 3 or first.dtype not in _capi.DTYPES:
+        raise ValueError(f"{what}: heads are bf16 or fp16 [T, H, D], got {first.dtype} {tuple(first.shape)}")
+    tokens, dim, dtype, device = first.size(0), first.size(2), first.dtype, first.device
+    for name, t in heads.items():
+        if t is not None and (t.dim() != 3 or t.size(0) != tokens or t.size(2) != dim or t.dtype != dtype
+                              or t.stride(2) != 1 or t.device != device):
+            raise ValueError(f"{what}: {name} is {t.dtype} {tuple(t.shape)} of strides {t.stride()} on {t.device}, not "
+                             f"{dtype} [{tokens}, H, {dim}] of unit dim stride on {device}")
+    if positions.dtype != torch.int64 or positions.shape != (tokens,) or not positions.is_contiguous():
+        raise ValueError(f"{what}: positions must be contiguous int64 [{tokens}], got {positions.dtype} "
+                         f"{tuple(positions.shape)}")
+    if (table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous() or table.size(0) < 1
+            or table.size(1) < 2 or table.size(1) % 2 or table.size(1) > dim):
+        raise ValueError(f"{what}: the table must be contiguous fp32 [positions, r] with r even and at most the head "
+                         f"width {dim}, got {table.dtype} {tuple(table.shape)}")
+    for name, w in weights.items():
+        if w is not None and (w.shape != (dim,) or w.dtype != dtype or w.stride(0) != 1 or w.device != device):
+            raise ValueError(f"{what}: {name} must be contiguous {dtype} [{dim}] on {device}, got {w.dtype} "
+                             f"{tuple(w.shape)} on {w.device}")
+    if positions.device != device or table.device != device or device.type != "cuda":
+        raise ValueError(f"{what}: heads on {device}, positions on {positions.device}, table on {table.device}; all must "
+                         "be on one GPU")
+    if checks.ENABLED:
+        checks.check_positions(positions, table.size(0))
+
+
+def head_args(t: torch.Tensor | None) -> tuple:
+    """Pointer, token stride and head stride of ``[T, H, D]`` (None: no heads)."""
+    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def apply_rotary(q, k, positions, table, interleaved: bool = False, out_q=None, out_k=None):
+    """Rotary positions on ``q`` ``[T, Hq, D]`` and ``k`` ``[T, Hkv, D]`` (either may be None), any token and head strides:
+    views of a fused projection, or of a part of each head, will do. ``positions`` int64 ``[T]``; ``table`` as
+    ``rotary_table`` makes it, of r <= D: the first r dims of each head turn in pairs ``(i, i + r / 2)``, or
+    ``(2 i, 2 i + 1)`` if ``interleaved``, the others are copied. Returns ``(q', k')``: new tensors, or ``out_q`` /
+    ``out_k``, each of which may be its input itself (in place) and must not overlap it otherwise. In fp32, rounded once.
+    A negative position rotates as position 0 (padding); one past the table gives NaN."""
+    return _rotate("apply_rotary", q, k, None, None, positions, table, 0.0, interleaved, out_q, out_k)
+
+
+def norm_rotary(q, k, q_weight, k_weight, positions, table, eps: float = 1e-6, interleaved: bool = False, out_q=None,
+                out_k=None):
+    """``apply_rotary`` on ``x * rsqrt(mean(x^2) + eps) * weight`` of every head, ``q_weight`` / ``k_weight`` ``[D]`` of the
+    heads' dtype (None: those heads are not normed), in the same pass and rounded only once."""
+    return _rotate("norm_rotary", q, k, q_weight, k_weight, positions, table, eps, interleaved, out_q, out_k)
+
+
+def _rotate(what, q, k, q_weight, k_weight, positions, table, eps, interleaved, out_q, out_k):
+    check_rotary(what, {"q": q, "k": k}, positions, table, {"q_weight": q_weight, "k_weight": k_weight})
+    first = q if q is not None else k
+    outs = []
+    for name, x, out in (("out_q", q, out_q), ("out_k", k, out_k)):
+        if out is None:
+            out = None if x is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        elif x is None or out.shape != x.shape or out.dtype != x.dtype or out.stride(2) != 1 or out.device != x.device:
+            raise ValueError(f"{what}: {name} is {out.dtype} {tuple(out.shape)} on {out.device}, not shaped and placed as "
+                             "its input, with unit dim stride")
+        outs.append(out)
+    out_q, out_k = outs
+    _capi.call_on(first.device, "lv_rotary", *head_args(q), *head_args(k), positions.data_ptr(), table.data_ptr(),
+                  table.size(0), table.size(1), int(interleaved), _capi.ptr(q_weight), _capi.ptr(k_weight), eps,
+                  first.size(0), 0 if q is None else q.size(1), 0 if k is None else k.size(1), first.size(2),
+                  *head_args(out_q), *head_args(out_k), _capi.DTYPES[first.dtype])
+    return out_q, out_k
