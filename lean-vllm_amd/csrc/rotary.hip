@@ -111,22 +111,240 @@ __global__ __launch_bounds__(256) void rotary_any_kernel(RotaryParams p, int32_t
   for (int d = p.rot + lane; d < p.dim; d += 64) store1<T>(r.dst, d, normed(d));
 }
 
+// Rows of whole 16-byte chunks: LPH lanes a head row, each two chunks that hold both elements of every pair in them (half
+// layout: chunks c and c + r / 16; interleaved, and behind the rotary width: c and the one as many further on as there
+// are such lanes, so that neighbouring lanes' chunks lie side by side: two adjacent chunks a lane took 43.3 us where
+// these take 37.3, 8192 tokens interleaved), so a row is read once, turned in registers and written once. A wave takes kRounds rounds of 64 / LPH head rows of one token,
+// their loads all issued before the first is used, and the table's 8 cosines and 8 sines a lane once for all rounds.
+//
+// Measured on 32/8 heads of 128, bf16, normed, into the cache: 8192 tokens 36.7 us, 5.60 TB/s (a 1 GiB copy: 5.25);
+// normed only, 16384 tokens 60.3 us, 5.71 TB/s; 1 to 100 tokens 4 us, a launch and three dependent loads (position, table
+// row, and under them the head rows). One, two, three and four rounds a wave: 8192 tokens 44.6 / 40.7 / 44.6 / 42.1 us.
+//
+// STREAM: loads and stores past the caches. A step's q, k and v come from the projection before and go to the attention
+// after, so a call that fits the 256 MB Infinity Cache leaves its outputs there; one that does not only evicts. A
+// projection's write, the append and a read of its outputs, cached / streamed: 12.6 MB 18.6 / 19.3 us, 100 MB 58.8 /
+// 60.9, 201 MB 122.1 / 113.2, 402 MB 233 / 220 (the append alone 40.7 / 36.7 at 201 MB). The line is drawn at 128 MB.
+constexpr int kRounds = 2;
+constexpr int64_t kStreamBytes = 128ll << 20;
+template <typename T, int LPH, bool INTERLEAVED, bool STREAM>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int32_t head_rows) {
+  using E = Elem<T>;
+  constexpr int NR = kRounds;
+  const int lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (t >= p.tokens) return;
+  const int64_t pos = p.positions[t];
+  const int lanes = p.dim / 16;  // lanes that hold a row
+  const bool holds = lane % LPH < lanes;
+  const int sub = holds ? lane % LPH : 0;
+  const int paired = INTERLEAVED ? 0 : p.rot / 16;  // lanes of the half layout's pairs of chunks
+  const int chunk_a = sub < paired ? sub : sub + paired, chunk_b = sub < paired ? sub + paired : sub + lanes;
+  const bool turns_a = 8 * chunk_a < p.rot, turns_b = 8 * chunk_b < p.rot;
+  const int ca = 16 * chunk_a, cb = 16 * chunk_b;  // bytes
+  HeadRow row[NR];
+  u32x4 xa[NR], xb[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int h = ((int)blockIdx.y * NR + r) * (64 / LPH) + lane / LPH;
+    row[r] = head_row(p, t, min(h, head_rows - 1));
+    if (h >= head_rows || !holds) row[r].dst = nullptr;
+    xa[r] = STREAM ? ld16_stream(row[r].src + ca) : ld16(row[r].src + ca);
+    xb[r] = STREAM ? ld16_stream(row[r].src + cb) : ld16(row[r].src + cb);
+  }
+  float amp;
+  const float* cosines = table_row(p, pos, amp);
+  // Half layout: the lane's eight pairs; interleaved: four in each chunk.
+  const int pa = turns_a ? (INTERLEAVED ? 4 * chunk_a : 8 * chunk_a) : 0;
+  const int pb = turns_b ? (INTERLEAVED ? 4 * chunk_b : 8 * chunk_a + 4) : 0;
+  float c[8], s[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    c[i] = cosines[pa + i], c[4 + i] = cosines[pb + i];
+    s[i] = cosines[p.rot / 2 + pa + i], s[4 + i] = cosines[p.rot / 2 + pb + i];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    c[i] *= amp;
+    s[i] *= amp;
+  }
+  const bool any_norm = p.q_weight || p.k_weight;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    float a[8], b[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[2 * i] = E::lo(xa[r][i]), a[2 * i + 1] = E::hi(xa[r][i]);
+      b[2 * i] = E::lo(xb[r][i]), b[2 * i + 1] = E::hi(xb[r][i]);
+    }
+    if (any_norm) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fmaf(a[i], a[i], fmaf(b[i], b[i], sum));
+      sum = holds ? sum : 0.f;
+      sum = group_sum<LPH>(sum);
+      if (row[r].weight) {
+        const float scale = rsqrtf(sum / (float)p.dim + p.eps);
+        const u32x4 wa = ld16(row[r].weight + ca), wb = ld16(row[r].weight + cb);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          a[2 * i] *= scale * E::lo(wa[i]), a[2 * i + 1] *= scale * E::hi(wa[i]);
+          b[2 * i] *= scale * E::lo(wb[i]), b[2 * i + 1] *= scale * E::hi(wb[i]);
+        }
+      }
+    }
+    u32x4 ya, yb;
+    if (!row[r].turned || (!turns_a && !row[r].weight)) {  // values, and dims that neither turn nor are normed: the bits
+      ya = xa[r];
+      yb = xb[r];
+    } else {
+      if constexpr (INTERLEAVED) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float a0 = a[2 * i], b0 = b[2 * i];
+          if (turns_a) {
+            a[2 * i] = a0 * c[i] - a[2 * i + 1] * s[i];
+            a[2 * i + 1] = a[2 * i + 1] * c[i] + a0 * s[i];
+          }
+          if (turns_b) {
+            b[2 * i] = b0 * c[4 + i] - b[2 * i + 1] * s[4 + i];
+            b[2 * i + 1] = b[2 * i + 1] * c[4 + i] + b0 * s[4 + i];
+          }
+        }
+      } else if (turns_a) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float a0 = a[i];
+          a[i] = a0 * c[i] - b[i] * s[i];
+          b[i] = b[i] * c[i] + a0 * s[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ya[i] = E::pack(a[2 * i], a[2 * i + 1]);
+        yb[i] = E::pack(b[2 * i], b[2 * i + 1]);
+      }
+    }
+    if (row[r].dst) {
+      if (STREAM) {
+        __builtin_nontemporal_store(ya, reinterpret_cast<u32x4*>(row[r].dst + ca));
+        __builtin_nontemporal_store(yb, reinterpret_cast<u32x4*>(row[r].dst + cb));
+      } else {
+        st16(row[r].dst + ca, ya);
+        st16(row[r].dst + cb, yb);
+      }
+    }
+  }
+}
+
+// The same rows with a rotary width that is no multiple of 16 (interleaved: 8), so that a pair's elements lie in other lanes (quarters
+// of 80- and 96-wide heads: 20 and 24): a lane holds two adjacent chunks and takes its elements' partners from the LDS. 8192 tokens, 32/8 heads of 80 of which 20 turn, normed
+// 52 us, rotary_any_kernel 140.
+template <typename T, int LPH>
+__global__ __launch_bounds__(256) void rotary_ragged_kernel(RotaryParams p, int32_t head_rows) {
+  using E = Elem<T>;
+  const int lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (t >= p.tokens) return;
+  const bool holds = lane % LPH < p.dim / 16;
+  const int d0 = holds ? lane % LPH * 16 : 0, half = p.rot / 2;
+  const int h = (int)blockIdx.y * (64 / LPH) + lane / LPH;
+  HeadRow row = head_row(p, t, min(h, head_rows - 1));
+  if (h >= head_rows || !holds) row.dst = nullptr;
+  u32x4 x[2] = {ld16(row.src + 2 * d0), ld16(row.src + 2 * d0 + 16)};
+  float e[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[2 * i] = E::lo(x[i / 4][i % 4]), e[2 * i + 1] = E::hi(x[i / 4][i % 4]);
+  if (p.q_weight || p.k_weight) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum = fmaf(e[i], e[i], sum);
+    sum = group_sum<LPH>(holds ? sum : 0.f);
+    if (row.weight) {
+      const float scale = rsqrtf(sum / (float)p.dim + p.eps);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const u32x4 w = ld16(row.weight + 2 * d0 + 16 * c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[8 * c + 2 * i] *= scale * E::lo(w[i]);
+          e[8 * c + 2 * i + 1] *= scale * E::hi(w[i]);
+        }
+      }
+    }
+  }
+  // 17 floats a lane, so that neighbours' i-th elements lie in different banks. A wave reads what it wrote.
+  __shared__ float held[4][64 * 17];
+  float* mine = held[threadIdx.x >> 6] + 17 * (lane - lane % LPH);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) mine[17 * (lane % LPH) + i] = e[i];
+  __builtin_amdgcn_wave_barrier();
+  if (row.turned && d0 < p.rot) {
+    float amp;
+    const float* row_table = table_row(p, p.positions[t], amp);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int d = min(d0 + i, p.rot - 1);
+      const bool second = p.interleaved ? d & 1 : d >= half;
+      const int pair = p.interleaved ? d / 2 : second ? d - half : d;
+      const int other = p.interleaved ? d ^ 1 : second ? pair : d + half;
+      const float y = mine[other + other / 16];
+      const float c = row_table[pair] * amp, s = row_table[half + pair] * amp;
+      if (d0 + i < p.rot) e[i] = second ? e[i] * c + y * s : e[i] * c - y * s;
+    }
+  }
+  if (row.turned && (row.weight || d0 < p.rot)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i / 4][i % 4] = E::pack(e[2 * i], e[2 * i + 1]);
+  }
+  if (row.dst) {
+    st16(row.dst + 2 * d0, x[0]);
+    st16(row.dst + 2 * d0 + 16, x[1]);
+  }
+}
+
+template <typename T, int LPH>
+static void launch_chunks(const RotaryParams& p, int32_t head_rows, hipStream_t stream) {
+  const int32_t rounds = (head_rows + 64 / LPH - 1) / (64 / LPH);
+  const uint32_t x = (uint32_t)((p.tokens + 3) / 4);
+  if (p.rot % (p.interleaved ? 8 : 16) != 0) {
+    hipLaunchKernelGGL((rotary_ragged_kernel<T, LPH>), dim3(x, rounds), dim3(256), 0, stream, p, head_rows);
+    return;
+  }
+  const bool stream_past = (int64_t)p.tokens * head_rows * p.dim * 4 > kStreamBytes;
+  auto* const kernel = p.interleaved ? (stream_past ? &rotary_kernel<T, LPH, true, true>
+                                                    : &rotary_kernel<T, LPH, true, false>)
+                                     : (stream_past ? &rotary_kernel<T, LPH, false, true>
+                                                    : &rotary_kernel<T, LPH, false, false>);
+  hipLaunchKernelGGL(kernel, dim3(x, (rounds + kRounds - 1) / kRounds), dim3(256), 0, stream, p, head_rows);
+}
+
 template <typename T>
 static int launch_rotary(const RotaryParams& p, hipStream_t stream) {
   const int32_t head_rows = p.hq + p.hkv * (p.slots ? 2 : 1);
   const int64_t wgs = ((int64_t)p.tokens * head_rows + 3) / 4;
   LV_REQUIRE(fits_one_launch(wgs, 256), "rotary: %d tokens of %d head rows need a grid larger than one launch holds",
              p.tokens, head_rows);
-  hipLaunchKernelGGL(rotary_any_kernel<T>, dim3((uint32_t)wgs), dim3(256), 0, stream, p, head_rows);
-  LV_LAUNCH_CHECK("rotary_any_kernel");
+  // Whole 16-byte chunks everywhere (the table's and the weights' alignment does not matter to the ragged kernel).
+  bool chunks = p.dim % 16 == 0 && p.dim <= 256 && aligned(p.q, 16) && aligned(p.k, 16) && aligned(p.v, 16) &&
+                aligned(p.q_out, 16) && aligned(p.k_out, 16) && aligned(p.v_cache, 16) && aligned(p.q_weight, 16) &&
+                aligned(p.k_weight, 16);
+  for (int64_t st : {p.q_st, p.q_sh, p.k_st, p.k_sh, p.v_st, p.v_sh, p.qo_st, p.qo_sh, p.ko_st, p.ko_sh, p.c_sb})
+    chunks = chunks && st % 16 == 0;
+  if (!chunks)
+    hipLaunchKernelGGL(rotary_any_kernel<T>, dim3((uint32_t)wgs), dim3(256), 0, stream, p, head_rows);
+  else if (p.dim <= 64) launch_chunks<T, 4>(p, head_rows, stream);
+  else if (p.dim <= 128) launch_chunks<T, 8>(p, head_rows, stream);
+  else launch_chunks<T, 16>(p, head_rows, stream);
+  LV_LAUNCH_CHECK("rotary kernel");
   return LV_OK;
 }
 
 // What both entry points require of the heads and the table.
 static int check_rotary(const char* what, const RotaryParams& p, int64_t max_position, int32_t dtype) {
   LV_REQUIRE(dtype == LV_DTYPE_BF16 || dtype == LV_DTYPE_F16, "%s: dtype %d is not bf16 or fp16", what, dtype);
-  LV_REQUIRE(p.tokens >= 0 && p.hq >= 0 && p.hkv >= 0 && p.hq + (int64_t)p.hkv > 0 && p.hq < (1 << 20) &&
-                 p.hkv < (1 << 20),
+  LV_REQUIRE(p.tokens >= 0 && p.hq >= 0 && p.hkv >= 0 && p.hq + (int64_t)p.hkv > 0 && p.hq <= (1 << 14) &&
+                 p.hkv <= (1 << 14),
              "%s: bad sizes T=%d Hq=%d Hkv=%d", what, p.tokens, p.hq, p.hkv);
   LV_REQUIRE(p.dim >= 2 && p.rot >= 2 && p.rot <= p.dim && p.rot % 2 == 0,
              "%s: the rotary width %d must be even and at most the head width %d", what, p.rot, p.dim);

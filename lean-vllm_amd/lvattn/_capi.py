@@ -132,13 +132,21 @@ def call(name: str, *args):
     return rc
 
 
-def call_on(device: torch.device, name: str, *args):
-    """``call`` on ``device``'s current stream (the C function's last argument), with ``device`` current: a launch and
+def _current_stream(device: int) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# The same handle without a Stream object, 0.1 us instead of 2.8 a call, where this torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
+
+
+def call_on(device: int, name: str, *args):
+    """``call`` on GPU ``device``'s current stream (the C function's last argument), with that GPU current: a launch and
     the library's per-device state go by the current device, which the tensors' need not be."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return call(name, *args, stream_of(device))
+    if device == torch.cuda.current_device():
+        return call(name, *args, _raw_stream(device))
     with torch.cuda.device(device):
-        return call(name, *args, stream_of(device))
+        return call(name, *args, _raw_stream(device))
 
 
 def query(name: str, *args):

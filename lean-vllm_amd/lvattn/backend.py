@@ -18,7 +18,7 @@ import torch
 from . import _capi, checks
 from .abstract import AttentionBackend
 from .context import Context
-from .rotary import check_rotary, head_args
+from .rotary import first_heads, head_args, output_heads, rotary_args
 
 
 def _arch_ok() -> bool:
@@ -150,34 +150,31 @@ class MI355XAttention(AttentionBackend):
         queries ``[T, Hq, D]`` (``out`` if given, which may be ``q`` itself). ``q``, ``k``, ``v`` ``[T, H, D]`` with any
         token and head strides; ``slot_mapping`` int32 ``[T]``, -1 storing nothing; ``positions`` and ``table`` as
         ``apply_rotary`` takes them. ``q`` None only fills the cache, and returns None."""
-        check_rotary("append_kvcache", {"k": k, "v": v, "q": q}, positions, table,
-                     {"q_weight": q_weight, "k_weight": k_weight})
-        tokens, heads, dim = k.shape
-        cs = k_cache.stride()
-        if (v.size(1) != heads or k_cache.dim() != 4 or k_cache.shape != v_cache.shape
-                or k_cache.shape[2:] != (heads, dim) or cs != v_cache.stride() or cs[3] != 1
-                or not k_cache.dtype == v_cache.dtype == k.dtype or not k_cache.device == v_cache.device == k.device):
-            raise ValueError(f"append_kvcache: keys {tuple(k.shape)} and values {tuple(v.shape)} of {k.dtype} on {k.device}"
-                             f" into caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} of {k_cache.dtype}, "
-                             f"{v_cache.dtype} on {k_cache.device}, {v_cache.device}")
-        if slot_mapping.shape != (tokens,) or slot_mapping.device != k.device:
-            raise ValueError(f"append_kvcache: {tuple(slot_mapping.shape)} slots on {slot_mapping.device} for {tokens} "
-                             f"tokens on {k.device}")
-        if q is not None and out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif out is not None and (q is None or out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1
-                                  or out.device != q.device):
-            raise ValueError(f"append_kvcache: out is {out.dtype} {tuple(out.shape)} on {out.device}, not shaped and "
-                             "placed as q, with unit dim stride")
-        if checks.ENABLED:
-            checks.check_slots(slot_mapping, k_cache.size(0), k_cache.size(1))
-        if slot_mapping.dtype != torch.int32 or not slot_mapping.is_contiguous():
+        what = "append_kvcache"
+        like = first_heads(what, k)
+        tokens, dim, dtype, device = like
+        *q_args, heads = head_args(what, "q", q, *like)
+        *k_args, kv_heads = head_args(what, "k", k, *like)
+        *v_args, v_heads = head_args(what, "v", v, *like)
+        pos, tab, held, width, qw, kw = rotary_args(what, positions, table, q_weight, k_weight, *like)
+        shape, cs = k_cache.shape, k_cache.stride()
+        if (v_heads != kv_heads or len(shape) != 4 or shape[2] != kv_heads or shape[3] != dim or shape != v_cache.shape
+                or cs != v_cache.stride() or cs[3] != 1 or not k_cache.dtype is v_cache.dtype is dtype
+                or not k_cache.get_device() == v_cache.get_device() == device):
+            raise ValueError(f"{what}: keys {tuple(k.shape)} and values {tuple(v.shape)} of {dtype} on {k.device} into "
+                             f"caches {tuple(shape)} and {tuple(v_cache.shape)} of {k_cache.dtype}, {v_cache.dtype}, "
+                             f"strides {cs}, {v_cache.stride()}, on {k_cache.device}, {v_cache.device}")
+        if slot_mapping.shape != (tokens,) or slot_mapping.get_device() != device:
+            raise ValueError(f"{what}: {tuple(slot_mapping.shape)} slots on {slot_mapping.device} for {tokens} tokens on "
+                             f"{k.device}")
+        if slot_mapping.dtype is not torch.int32 or not slot_mapping.is_contiguous():
             slot_mapping = slot_mapping.to(torch.int32).contiguous()
-        _capi.call_on(k.device, "lv_append_kvcache", *head_args(q), *head_args(k), *head_args(v), positions.data_ptr(),
-                      table.data_ptr(), table.size(0), table.size(1), int(interleaved), _capi.ptr(q_weight),
-                      _capi.ptr(k_weight), eps, tokens, 0 if q is None else q.size(1), heads, dim, *head_args(out),
-                      k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], k_cache.size(1),
-                      slot_mapping.data_ptr(), _capi.DTYPES[k.dtype])
+        out, o_args = output_heads(what, "out", q, out, like)
+        if checks.ENABLED:
+            checks.check_slots(slot_mapping, shape[0], shape[1])
+        _capi.call_on(device, "lv_append_kvcache", *q_args, *k_args, *v_args, pos, tab, held, width, interleaved, qw, kw,
+                      eps, tokens, heads, kv_heads, dim, *o_args, k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1],
+                      cs[2], shape[1], slot_mapping.data_ptr(), _capi.DTYPES[dtype])
         return out
 
     def store_latents(self, latent, latent_cache, slot_mapping) -> None:

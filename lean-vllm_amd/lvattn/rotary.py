@@ -88,42 +88,63 @@ def rotary_table(rotary_dim: int, max_position: int, base: float = 10000.0, scal
     return table
 
 
-def check_rotary(what: str, heads: dict, positions, table, weights: dict) -> None:
-    """Raises ``ValueError`` unless every tensor of ``heads`` (name -> ``[T, H, D]`` or None) has the same T, D, dtype and
-    unit dim stride, ``positions`` is int64 ``[T]``, ``table`` fp32 ``[P, r]`` with r even and at most D, the ``weights``
-    ``[D]`` of the heads' dtype, and all are on one GPU."""
-    first = next((t for t in heads.values() if t is not None), None)
-    if first is None:
-        raise ValueError(f"{what}: no heads to rotate")
-    if first.dim() != 3 or first.dtype not in _capi.DTYPES:
-        raise ValueError(f"{what}: heads are bf16 or fp16 [T, H, D], got {first.dtype} {tuple(first.shape)}")
-    tokens, dim, dtype, device = first.size(0), first.size(2), first.dtype, first.device
-    for name, t in heads.items():
-        if t is not None and (t.dim() != 3 or t.size(0) != tokens or t.size(2) != dim or t.dtype != dtype
-                              or t.stride(2) != 1 or t.device != device):
-            raise ValueError(f"{what}: {name} is {t.dtype} {tuple(t.shape)} of strides {t.stride()} on {t.device}, not "
-                             f"{dtype} [{tokens}, H, {dim}] of unit dim stride on {device}")
-    if positions.dtype != torch.int64 or positions.shape != (tokens,) or not positions.is_contiguous():
+def head_args(what: str, name: str, t, tokens: int, dim: int, dtype, device: int) -> tuple:
+    """Pointer, token stride, head stride and heads of ``t`` ``[T, H, D]`` for the C call (None: no heads). Raises
+    ``ValueError`` unless it has ``tokens``, ``dim``, ``dtype``, a unit dim stride and lies on GPU ``device``."""
+    if t is None:
+        return None, 0, 0, 0
+    shape, stride = t.shape, t.stride()
+    if (len(shape) != 3 or shape[0] != tokens or shape[2] != dim or stride[2] != 1 or t.dtype is not dtype
+            or t.get_device() != device):
+        raise ValueError(f"{what}: {name} is {t.dtype} {tuple(shape)} of strides {stride} on {t.device}, not {dtype} "
+                         f"[{tokens}, H, {dim}] of unit dim stride beside the other heads")
+    return t.data_ptr(), stride[0], stride[1], shape[1]
+
+
+def rotary_args(what: str, positions, table, q_weight, k_weight, tokens: int, dim: int, dtype, device: int) -> tuple:
+    """The C call's positions, table and weights. Raises ``ValueError`` unless ``positions`` is contiguous int64 ``[T]``,
+    ``table`` contiguous fp32 ``[P, r]`` with r even and at most D, the weights contiguous ``[D]`` of the heads' dtype, and
+    all on GPU ``device``."""
+    if positions.dtype is not torch.int64 or positions.shape != (tokens,) or not positions.is_contiguous():
         raise ValueError(f"{what}: positions must be contiguous int64 [{tokens}], got {positions.dtype} "
                          f"{tuple(positions.shape)}")
-    if (table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous() or table.size(0) < 1
-            or table.size(1) < 2 or table.size(1) % 2 or table.size(1) > dim):
+    shape = table.shape
+    if (len(shape) != 2 or table.dtype is not torch.float32 or shape[0] < 1 or shape[1] < 2 or shape[1] % 2
+            or shape[1] > dim or not table.is_contiguous()):
         raise ValueError(f"{what}: the table must be contiguous fp32 [positions, r] with r even and at most the head "
-                         f"width {dim}, got {table.dtype} {tuple(table.shape)}")
-    for name, w in weights.items():
-        if w is not None and (w.shape != (dim,) or w.dtype != dtype or w.stride(0) != 1 or w.device != device):
-            raise ValueError(f"{what}: {name} must be contiguous {dtype} [{dim}] on {device}, got {w.dtype} "
+                         f"width {dim}, got {table.dtype} {tuple(shape)}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (w.shape != (dim,) or w.dtype is not dtype or not w.is_contiguous()
+                              or w.get_device() != device):
+            raise ValueError(f"{what}: {name} must be contiguous {dtype} [{dim}] beside the heads, got {w.dtype} "
                              f"{tuple(w.shape)} on {w.device}")
-    if positions.device != device or table.device != device or device.type != "cuda":
-        raise ValueError(f"{what}: heads on {device}, positions on {positions.device}, table on {table.device}; all must "
-                         "be on one GPU")
+    if device < 0 or positions.get_device() != device or table.get_device() != device:
+        raise ValueError(f"{what}: positions on {positions.device}, table on {table.device}, heads on GPU {device}; all "
+                         "must be on one GPU")
     if checks.ENABLED:
-        checks.check_positions(positions, table.size(0))
+        checks.check_positions(positions, shape[0])
+    return positions.data_ptr(), table.data_ptr(), shape[0], shape[1], _capi.ptr(q_weight), _capi.ptr(k_weight)
 
 
-def head_args(t: torch.Tensor | None) -> tuple:
-    """Pointer, token stride and head stride of ``[T, H, D]`` (None: no heads)."""
-    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+def first_heads(what: str, t) -> tuple:
+    """Tokens, width, dtype and GPU of the heads that the others have to match."""
+    if t.dim() != 3 or t.dtype not in _capi.DTYPES:
+        raise ValueError(f"{what}: heads are bf16 or fp16 [T, H, D], got {t.dtype} {tuple(t.shape)}")
+    tokens, _, dim = t.shape
+    return tokens, dim, t.dtype, t.get_device()
+
+
+def output_heads(what: str, name: str, x, out, like: tuple):
+    """``out``, checked against its input ``x`` ``[T, H, D]``, or a new tensor; and its arguments for the C call."""
+    if out is None:
+        if x is None:
+            return None, (None, 0, 0)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        return out, (out.data_ptr(), x.size(1) * like[1], like[1])
+    if x is None or out.shape != x.shape:
+        raise ValueError(f"{what}: {name} is {tuple(out.shape)}, its input "
+                         f"{'missing' if x is None else tuple(x.shape)}")
+    return out, head_args(what, name, out, *like)[:3]
 
 
 def apply_rotary(q, k, positions, table, interleaved: bool = False, out_q=None, out_k=None):
@@ -144,19 +165,15 @@ def norm_rotary(q, k, q_weight, k_weight, positions, table, eps: float = 1e-6, i
 
 
 def _rotate(what, q, k, q_weight, k_weight, positions, table, eps, interleaved, out_q, out_k):
-    check_rotary(what, {"q": q, "k": k}, positions, table, {"q_weight": q_weight, "k_weight": k_weight})
-    first = q if q is not None else k
-    outs = []
-    for name, x, out in (("out_q", q, out_q), ("out_k", k, out_k)):
-        if out is None:
-            out = None if x is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        elif x is None or out.shape != x.shape or out.dtype != x.dtype or out.stride(2) != 1 or out.device != x.device:
-            raise ValueError(f"{what}: {name} is {out.dtype} {tuple(out.shape)} on {out.device}, not shaped and placed as "
-                             "its input, with unit dim stride")
-        outs.append(out)
-    out_q, out_k = outs
-    _capi.call_on(first.device, "lv_rotary", *head_args(q), *head_args(k), positions.data_ptr(), table.data_ptr(),
-                  table.size(0), table.size(1), int(interleaved), _capi.ptr(q_weight), _capi.ptr(k_weight), eps,
-                  first.size(0), 0 if q is None else q.size(1), 0 if k is None else k.size(1), first.size(2),
-                  *head_args(out_q), *head_args(out_k), _capi.DTYPES[first.dtype])
+    if q is None and k is None:
+        raise ValueError(f"{what}: no heads to rotate")
+    like = first_heads(what, q if q is not None else k)
+    tokens, dim, dtype, device = like
+    *q_args, heads = head_args(what, "q", q, *like)
+    *k_args, kv_heads = head_args(what, "k", k, *like)
+    pos, tab, positions_held, width, qw, kw = rotary_args(what, positions, table, q_weight, k_weight, *like)
+    out_q, oq_args = output_heads(what, "out_q", q, out_q, like)
+    out_k, ok_args = output_heads(what, "out_k", k, out_k, like)
+    _capi.call_on(device, "lv_rotary", *q_args, *k_args, pos, tab, positions_held, width, interleaved, qw, kw, eps, tokens,
+                  heads, kv_heads, dim, *oq_args, *ok_args, _capi.DTYPES[dtype])
     return out_q, out_k

@@ -43,7 +43,8 @@ CASES = [  # tokens, heads, kv heads, dim, rotary dim, pad
     (33, 8, 8, 256, 64, 0), (18, 5, 3, 96, 96, 0), (70, 16, 2, 80, 80, 8), (19, 16, 2, 80, 32, 0), (5, 4, 2, 192, 192, 0),
     (9, 3, 1, 512, 512, 0), (7, 2, 1, 576, 64, 0), (6, 2, 1, 1024, 128, 0),
     (21, 5, 1, 128, 128, 1), (11, 3, 2, 80, 20, 0), (8, 2, 2, 6, 4, 0), (130, 1, 1, 2, 2, 0), (2, 3, 1, 130, 66, 3),
-    (900, 2, 1, 64, 16, 4),
+    (900, 2, 1, 64, 16, 4), (13, 5, 2, 96, 24, 0), (9, 6, 2, 64, 20, 0), (5, 2, 1, 256, 40, 0), (4, 2, 1, 512, 18, 0),
+    (3, 2, 1, 1024, 100, 0),
 ]
 
 
@@ -76,6 +77,32 @@ def test_rotary_and_norm_match_the_oracle(cuda, t, hq, hk, dim, rot, pad, dtype,
     plain_k = lvattn.apply_rotary(None, dk, positions.to(cuda), table, interleaved=interleaved)
     assert plain_k[0] is None and torch.equal(iq, got[0]) and torch.equal(ik, plain_k[1])
     assert torch.equal(in_place[:, (hq + hk) * dim:].cpu(), kept)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_a_call_larger_than_the_cache_gives_the_bits_of_its_parts(cuda, dim, dtype, interleaved):
+    """Past 128 MB read and written the chunks go past the caches: the same bits as token ranges on their own."""
+    hq, hk, bs = 4, 2, 32
+    t = (130 << 20) // ((hq + 2 * hk) * dim * 4)
+    gen = torch.Generator(device=cuda).manual_seed(dim)
+    x = torch.randn(t, (hq + 2 * hk) * dim, device=cuda, generator=gen).to(dtype)
+    q, k, v = (y.view(t, -1, dim) for y in x.split([hq * dim, hk * dim, hk * dim], 1))
+    pos = torch.randint(0, 5000, (t,), device=cuda, generator=gen)
+    slots = torch.randperm((t // bs + 2) * bs, device=cuda, generator=gen)[:t].int()
+    w, table = torch.randn(dim, device=cuda, generator=gen).to(dtype), lvattn.rotary_table(dim, 5000, device=cuda)
+    backend = lvattn.MI355XAttention(hq, dim, 1.0, hk)
+    runs = []
+    for step in (t, t // 3 + 1):
+        caches = [torch.zeros(t // bs + 2, bs, hk, dim, dtype=dtype, device=cuda) for _ in range(2)]
+        outs = [backend.append_kvcache(q[a:a + step], k[a:a + step], v[a:a + step], *caches, slots[a:a + step],
+                                       pos[a:a + step], table, q_weight=w, k_weight=w, interleaved=interleaved)
+                for a in range(0, t, step)]
+        runs.append((torch.cat(outs), *caches))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    close(runs[0][0][-2:], *R.rotate(q[-2:].cpu(), pos[-2:].cpu(), dim, weight=w.cpu(), eps=EPS,
+                                        interleaved=interleaved))
 
 
 def test_odd_positions(cuda):
