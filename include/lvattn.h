@@ -240,6 +240,35 @@ int lv_paged_attention_static(const void* q, int64_t q_stride_t, int64_t q_strid
                               void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------
+ * Decode of rows that share their leading keys: lv_paged_attention's result for such a step (one query per row, or the
+ * queries_per_row last positions of each), with the shared keys read once for all rows instead of once for each. No
+ * counterpart in the reference, whose backends attend every row by itself (lean_vllm/attention/abstract.py:166-176).
+ *
+ * The first shared_len keys of every row lie in the pages that row 0's table begins with; shared_len is whole pages, at
+ * most max_seqlen_k. context_lens[num_rows] counts a row's keys, shared and own; query j sees keys
+ * 0 .. context_lens - queries_per_row + j. The rows' tables are whole (their shared entries are not read, except row 0's
+ * and those of a row whose first query does not see all shared keys: that row is attended by itself, through its own
+ * table). A row of no keys (graph padding) gets zeros. A value that is NaN or infinite makes its dim NaN or infinite in
+ * the rows that see it, and in no other.
+ * q, out: [num_rows * queries_per_row, num_heads, head_dim], row b's queries consecutive; strides, caches, tables and
+ * max_seqlen_k as lv_paged_attention's. head_dim 64 or 128; queries_per_row times query heads per kv head at most 64;
+ * pages of a multiple of 16.
+ * workspace: at least lv_shared_prefix_workspace_bytes(...) bytes for the same arguments, 256-byte aligned; no
+ * initialisation needed and nothing kept in it, but it must not be one that holds a step's plan
+ * (LV_ATTN_REUSE_PLAN). */
+size_t lv_shared_prefix_workspace_bytes(int32_t num_rows, int32_t queries_per_row, int32_t num_heads,
+                                        int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t shared_len,
+                                        int32_t max_seqlen_k);
+int lv_shared_prefix_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
+                            const void* v_cache, int64_t cache_stride_block, int64_t cache_stride_token,
+                            int64_t cache_stride_head, int32_t block_size, const int32_t* block_tables,
+                            int64_t table_stride, const int32_t* context_lens, int32_t num_rows,
+                            int32_t queries_per_row, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                            float scale, int32_t shared_len, int32_t max_seqlen_k, void* out, int64_t out_stride_t,
+                            int64_t out_stride_h, void* workspace, size_t workspace_bytes, int32_t dtype,
+                            void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
  * Attention over packed keys (no pages). Replaces AttentionBackend.prefill without block tables and
  * AttentionBackend.varlen_with_lse (lean_vllm/attention/abstract.py:148-164,187-204; math of TorchAttention.prefill
  * and varlen_with_lse, lean_vllm/attention/torch_backend.py:62-91): the warmup prefill and MLA prefill chunks.

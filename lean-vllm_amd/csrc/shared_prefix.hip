@@ -1,0 +1,307 @@
+// Decode of rows whose leading keys lie in the same pages (a system prompt, a document, samples of one prompt): the
+// shared keys attended once for all rows, each row's own keys by itself, joined by log-sum-exp.
+//
+// A query that sees keys 0 .. L - 1, the first P of them shared, has o = sum_j e^(s_j) v_j / sum_j e^(s_j). Cut into ranges
+// of keys with partial outputs o_i and log-sum-exps l_i it is sum_i e^(l_i - M) o_i / sum_i e^(l_i - M) for any M, so the
+// shared ranges can be walked with every row's queries together: their keys are read rows times less often than by
+// lv_paged_attention (math of TorchAttention.decode, lean_vllm/attention/torch_backend.py:93-103, row by row).
+//
+// Three launches: the prefix (query tiles x kv heads x pieces of its keys), the rows' own keys (rows x kv heads x splits),
+// and the merge of the fp32 partials. Everything is sized by the host from shapes and bounds; the rows' lengths are read
+// on the device, so a call can be captured.
+#include "few_item.h"
+
+namespace lv {
+
+constexpr int kSharedRound = 512;    // workgroups that run at once (two per CU)
+constexpr int kOwnKeys = 256;        // least keys a row's own split is cut for
+constexpr int kSharedPieceKeys = 256;  // and a piece of the prefix
+constexpr int kMaxOwnSplits = 32;
+constexpr int kMaxSharedPieces = 64;
+
+struct SharedParams : AttnParams {
+  int32_t shared, queries, tokens;  // keys of the prefix; queries per row; all queries
+  int32_t tile_rows, tiles;         // (query, head) rows of a prefix tile, tiles per kv head
+  int32_t per_piece, splits;        // keys per piece (p.pieces of them); most splits of a row's own keys
+};
+
+// A row's own part: its keys from `start` on, in `n` splits of `per` (none where the row has no keys). A row that does not
+// see the whole prefix (its first query sees fewer keys) is attended by itself from key 0 on.
+struct OwnSpan {
+  int start, per, n;
+};
+__device__ __forceinline__ OwnSpan own_span(const SharedParams& p, int len) {
+  OwnSpan s;
+  s.start = len - p.queries + 1 >= p.shared ? p.shared : 0;
+  const int keys = len - s.start;
+  const int want = min(p.splits, (keys + kOwnKeys - 1) / kOwnKeys);
+  s.per = want > 1 ? ((keys + want - 1) / want + 63) / 64 * 64 : max(keys, 1);
+  s.n = keys > 0 ? (keys + s.per - 1) / s.per : 0;
+  return s;
+}
+
+// Partials lie by slot: piece i of token t's prefix in slot i tokens + t, its row's own split j in slot
+// (pieces + j) tokens + t.
+template <typename T, int D, int NB, FewSets SETS>
+__global__ __launch_bounds__(64 * kWaves, 2) void shared_own_kernel(SharedParams p) {
+  __shared__ __attribute__((aligned(16))) char smem[kWaves * kFewStages * kFewStage];
+  const int kvh = blockIdx.x % p.hkv, i = blockIdx.x / p.hkv;
+  const int split = i / p.rows, row = i - split * p.rows;
+  const int len = sload(p.lens_k + row);
+  const OwnSpan s = own_span(p, len);
+  if (split >= s.n) return;
+  FewPart part;
+  part.table = p.tables + (int64_t)row * p.t_stride;
+  part.lk = len;
+  part.lq = p.queries;
+  part.tok = row * p.queries;
+  part.kbeg = s.start + split * s.per;
+  part.kend = min(len, part.kbeg + s.per);
+  part.row0 = 0;
+  part.row_end = p.queries * p.group;
+  part.slot0 = (p.pieces + split) * p.tokens + part.tok;
+  part.causal = true;
+  few_item<T, D, NB, SETS, true>(p, row, 0, 0, kvh, smem, part);
+}
+
+template <typename T, int D, int NB, FewSets SETS>
+__global__ __launch_bounds__(64 * kWaves, 2) void shared_prefix_kernel(SharedParams p) {
+  __shared__ __attribute__((aligned(16))) char smem[kWaves * kFewStages * kFewStage];
+  const int kvh = blockIdx.x % p.hkv, i = blockIdx.x / p.hkv;
+  const int piece = i / p.tiles, tile = i - piece * p.tiles;
+  FewPart part;
+  part.table = p.tables;
+  part.lk = p.shared;
+  part.lq = p.tokens;
+  part.tok = 0;
+  part.kbeg = piece * p.per_piece;
+  part.kend = min(p.shared, part.kbeg + p.per_piece);
+  part.row0 = tile * p.tile_rows;
+  part.row_end = min(p.tokens * p.group, part.row0 + p.tile_rows);
+  part.slot0 = piece * p.tokens;
+  part.causal = false;
+  few_item<T, D, NB, SETS, true>(p, 0, 0, 0, kvh, smem, part);
+}
+
+// One workgroup per (token, head): D / 4 threads a partial, 256 / (D / 4) partials at a time, joined through LDS.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void shared_merge_kernel(SharedParams p) {
+  using E = Elem<T>;
+  constexpr int LPR = D / 4, GROUPS = 256 / LPR, BATCH = 4;
+  __shared__ float part[GROUPS][D + 2];
+  const int tok = blockIdx.x / p.hq, head = blockIdx.x - tok * p.hq;
+  const int g = threadIdx.x / LPR, d0 = threadIdx.x % LPR * 4;
+  const int len = sload(p.lens_k + tok / p.queries);
+  const OwnSpan s = own_span(p, len);
+  const int shared = s.start > 0 ? p.pieces : 0;  // the partials: so many of the prefix, then s.n
+  const int count = shared + s.n;
+  float m = -INFINITY, den = 0.f;
+  f32x4 o = {0, 0, 0, 0};
+  for (int e0 = g; e0 < count; e0 += GROUPS * BATCH) {
+    float ls[BATCH];
+    f32x4 x[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int e = e0 + i * GROUPS;
+      ls[i] = -INFINITY;
+      x[i] = f32x4{0, 0, 0, 0};
+      if (e < count) {
+        const int64_t at = ((int64_t)(e < shared ? e : p.pieces + e - shared) * p.tokens + tok) * p.hq + head;
+        ls[i] = p.part_lse[at];
+        x[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + d0);
+      }
+    }
+    float bm = m;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) bm = fmaxf(bm, ls[i]);
+    const float base = merge_base(bm), alpha = fast_exp2(m - base);
+    den *= alpha;
+    o *= alpha;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const float w = fast_exp2(ls[i] - base);
+      den += w;
+      o += w * x[i];
+    }
+    m = bm;
+  }
+  *reinterpret_cast<f32x4*>(&part[g][d0]) = o;
+  if (d0 == 0) part[g][D] = m, part[g][D + 1] = den;
+  __syncthreads();
+  if (g > 0) return;
+  float bm = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) bm = fmaxf(bm, part[i][D]);
+  const float base = merge_base(bm);
+  den = 0.f;
+  o = f32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    const float w = fast_exp2(part[i][D] - base);
+    den += w * part[i][D + 1];
+    o += w * *reinterpret_cast<const f32x4*>(&part[i][d0]);
+  }
+  o *= inv_sum(den);
+  *reinterpret_cast<u32x2*>(p.out + (int64_t)tok * p.o_st + (int64_t)head * p.o_sh + d0 * 2) =
+      u32x2{E::pack(o[0], o[1]), E::pack(o[2], o[3])};
+}
+
+// What the host decides from the shapes.
+struct SharedPlan {
+  int32_t tile_rows, tiles, pieces, per_piece, splits;
+  size_t o_bytes, bytes;  // partial outputs, then their log-sum-exps
+};
+
+// (query, head) rows of a few-query item, by how many there are.
+static int few_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+static SharedPlan shared_plan(int32_t rows, int32_t queries, int32_t hq, int32_t hkv, int32_t d, int32_t shared,
+                              int32_t max_k) {
+  SharedPlan s{};
+  const int group = hq / hkv;
+  const int64_t tokens = (int64_t)rows * queries, query_rows = tokens * group;
+  s.tile_rows = few_rows(query_rows);
+  s.tiles = (int32_t)((query_rows + s.tile_rows - 1) / s.tile_rows);
+  s.per_piece = 64;
+  if (shared > 0) {
+    const int64_t units = (int64_t)s.tiles * hkv;
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>({kSharedRound / units, kMaxSharedPieces,
+                                                                 shared / kSharedPieceKeys}));
+    s.per_piece = (int32_t)(((shared + want - 1) / want + 63) / 64 * 64);
+    s.pieces = (shared + s.per_piece - 1) / s.per_piece;
+  }
+  // A row that does not see the prefix walks all its keys, so the bound is on those, not on the keys behind it.
+  const int64_t units = (int64_t)rows * hkv;
+  s.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({(kSharedRound + units - 1) / units, kMaxOwnSplits,
+                                                              ((int64_t)max_k + kOwnKeys - 1) / kOwnKeys}));
+  const int64_t partials = ((int64_t)s.pieces + s.splits) * tokens * hq;
+  s.o_bytes = (size_t)partials * d * sizeof(float);
+  s.bytes = s.o_bytes + (size_t)partials * sizeof(float);
+  return s;
+}
+
+template <typename T, int D, int NB, FewSets SETS>
+static void launch_few(const SharedParams& p, bool prefix, hipStream_t stream) {
+  const dim3 block(64 * kWaves);
+  if (prefix)
+    hipLaunchKernelGGL((shared_prefix_kernel<T, D, NB, SETS>), dim3(p.pieces * p.tiles * p.hkv), block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((shared_own_kernel<T, D, NB, SETS>), dim3(p.splits * p.rows * p.hkv), block, 0, stream, p);
+}
+
+template <typename T, int D>
+static int launch_shared(const SharedParams& p, hipStream_t stream) {
+  for (int prefix = p.pieces > 0; prefix >= 0; --prefix) {
+    const int rows = prefix ? p.tile_rows : few_rows(p.queries * p.group);
+    if (rows <= 16) launch_few<T, D, 1, kOneSet>(p, prefix, stream);
+    else if (rows <= 32) launch_few<T, D, 2, kOneSet>(p, prefix, stream);
+    else launch_few<T, D, (D == 64 ? 4 : 2), (D == 64 ? kOneSet : kTwoBlocks)>(p, prefix, stream);
+    LV_LAUNCH_CHECK("shared-prefix attention kernel");
+  }
+  hipLaunchKernelGGL((shared_merge_kernel<T, D>), dim3(p.tokens * p.hq), dim3(256), 0, stream, p);
+  LV_LAUNCH_CHECK("shared_merge_kernel");
+  return LV_OK;
+}
+
+static int check_shared(int32_t rows, int32_t queries, int32_t hq, int32_t hkv, int32_t d, int32_t block_size,
+                        int32_t shared, int32_t max_k) {
+  LV_REQUIRE(rows >= 0 && queries > 0, "shared_prefix_decode: bad sizes rows=%d queries=%d", rows, queries);
+  LV_REQUIRE(hq > 0 && hkv > 0 && hq % hkv == 0, "shared_prefix_decode: %d query heads do not group over %d key heads",
+             hq, hkv);
+  LV_REQUIRE(d == 64 || d == 128, "shared_prefix_decode: head_dim %d is not 64 or 128", d);
+  LV_REQUIRE((int64_t)queries * (hq / hkv) <= kFewMaxRows,
+             "shared_prefix_decode: %d queries of %d heads a key head; at most %d together", queries, hq / hkv,
+             kFewMaxRows);
+  LV_REQUIRE(block_size > 0 && block_size % 16 == 0, "shared_prefix_decode: page size %d is not a multiple of 16",
+             block_size);
+  LV_REQUIRE(max_k >= 0 && max_k <= (1 << 30), "shared_prefix_decode: max_seqlen_k %d is negative or above 2^30 keys",
+             max_k);
+  LV_REQUIRE(shared >= 0 && shared <= max_k && shared % block_size == 0,
+             "shared_prefix_decode: %d shared keys are not whole pages of %d within max_seqlen_k %d", shared, block_size,
+             max_k);
+  const int64_t tokens = (int64_t)rows * queries;
+  LV_REQUIRE(fits_one_launch(tokens * hq, 256) && fits_one_launch((int64_t)rows * hkv * kMaxOwnSplits, 256) &&
+                 tokens * hq * (kMaxOwnSplits + kMaxSharedPieces) < (int64_t)1 << 31,
+             "shared_prefix_decode: %lld queries of %d heads are more than one launch holds", (long long)tokens, hq);
+  return LV_OK;
+}
+
+}  // namespace lv
+
+using namespace lv;
+
+extern "C" size_t lv_shared_prefix_workspace_bytes(int32_t num_rows, int32_t queries_per_row, int32_t num_heads,
+                                                   int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                                   int32_t shared_len, int32_t max_seqlen_k) {
+  if (num_rows <= 0 || check_shared(num_rows, queries_per_row, num_heads, num_kv_heads, head_dim, block_size,
+                                    shared_len, max_seqlen_k) != LV_OK)
+    return 0;
+  return shared_plan(num_rows, queries_per_row, num_heads, num_kv_heads, head_dim, shared_len, max_seqlen_k).bytes;
+}
+
+extern "C" int lv_shared_prefix_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
+                                       const void* v_cache, int64_t cache_stride_block, int64_t cache_stride_token,
+                                       int64_t cache_stride_head, int32_t block_size, const int32_t* block_tables,
+                                       int64_t table_stride, const int32_t* context_lens, int32_t num_rows,
+                                       int32_t queries_per_row, int32_t num_heads, int32_t num_kv_heads,
+                                       int32_t head_dim, float scale, int32_t shared_len, int32_t max_seqlen_k,
+                                       void* out, int64_t out_stride_t, int64_t out_stride_h, void* workspace,
+                                       size_t workspace_bytes, int32_t dtype, void* stream) {
+  LV_REQUIRE(dtype == LV_DTYPE_BF16 || dtype == LV_DTYPE_F16, "shared_prefix_decode: dtype %d is not bf16 or fp16",
+             dtype);
+  const int rc = check_shared(num_rows, queries_per_row, num_heads, num_kv_heads, head_dim, block_size, shared_len,
+                              max_seqlen_k);
+  if (rc != LV_OK || num_rows == 0) return rc;
+  LV_REQUIRE(q && k_cache && v_cache && out && context_lens && (block_tables || max_seqlen_k == 0),
+             "shared_prefix_decode: null tensor pointer");
+  LV_REQUIRE(aligned(q, 16) && aligned(out, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) &&
+                 (q_stride_t * 2) % 16 == 0 && (q_stride_h * 2) % 16 == 0 && (out_stride_t * 2) % 16 == 0 &&
+                 (out_stride_h * 2) % 16 == 0 && (cache_stride_block * 2) % 16 == 0 &&
+                 (cache_stride_token * 2) % 16 == 0 && (cache_stride_head * 2) % 16 == 0,
+             "shared_prefix_decode: tensors and their strides must be 16-byte aligned");
+  LV_REQUIRE(cache_stride_token >= 0 && (int64_t)kPrefillKeys * cache_stride_token * 2 < (int64_t)1 << 30,
+             "shared_prefix_decode: cache token stride %lld is negative or too large", (long long)cache_stride_token);
+  LV_REQUIRE(scale > 0.f, "shared_prefix_decode: the softmax scale must be positive, got %g", (double)scale);
+  const SharedPlan s =
+      shared_plan(num_rows, queries_per_row, num_heads, num_kv_heads, head_dim, shared_len, max_seqlen_k);
+  LV_REQUIRE(workspace && workspace_bytes >= s.bytes, "shared_prefix_decode: workspace of %zu bytes given, %zu needed",
+             workspace_bytes, s.bytes);
+  LV_REQUIRE(aligned(workspace, 256), "shared_prefix_decode: workspace must be 256-byte aligned");
+  SharedParams p{};
+  p.q = (const char*)q;
+  p.q_st = q_stride_t * 2;
+  p.q_sh = q_stride_h * 2;
+  p.k_cache = (const char*)k_cache;
+  p.v_cache = (const char*)v_cache;
+  p.c_sb = cache_stride_block * 2;
+  p.c_st = p.v_st = cache_stride_token * 2;
+  p.c_sh = p.v_sh = cache_stride_head * 2;
+  p.paged = true;
+  p.bs = FastDiv::make(block_size);
+  p.tables = block_tables;
+  p.t_stride = table_stride;
+  p.lens_k = context_lens;
+  p.rows = num_rows;
+  p.hq = num_heads;
+  p.hkv = num_kv_heads;
+  p.group = num_heads / num_kv_heads;
+  p.qgroups = 1;
+  p.scale_log2 = scale * kLog2e;
+  p.out = (char*)out;
+  p.o_st = out_stride_t * 2;
+  p.o_sh = out_stride_h * 2;
+  p.part_o = (float*)workspace;
+  p.part_lse = (float*)((char*)workspace + s.o_bytes);
+  p.pieces = s.pieces;
+  p.shared = shared_len;
+  p.queries = queries_per_row;
+  p.tokens = num_rows * queries_per_row;
+  p.tile_rows = s.tile_rows;
+  p.tiles = s.tiles;
+  p.per_piece = s.per_piece;
+  p.splits = s.splits;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == LV_DTYPE_BF16)
+    return head_dim == 64 ? launch_shared<BF16, 64>(p, st) : launch_shared<BF16, 128>(p, st);
+  return head_dim == 64 ? launch_shared<F16, 64>(p, st) : launch_shared<F16, 128>(p, st);
+}

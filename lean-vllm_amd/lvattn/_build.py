@@ -20,7 +20,7 @@ INCLUDE = PACKAGE_DIR.parent.parent / "include"
 LIBRARY = PACKAGE_DIR / "liblvattn.so"
 BUILD_DIR = PACKAGE_DIR.parent / "_build"
 SOURCES = ("capi.hip", "store.hip", "pack.hip", "paged_attention.hip", "few_query.hip", "merge.hip", "mla_decode.hip", "varlen.hip",
-           "rotary.hip")
+           "rotary.hip", "shared_prefix.hip")
 ARCH = "gfx950"
 
 

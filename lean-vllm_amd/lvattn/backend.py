@@ -323,6 +323,57 @@ class MI355XAttention(AttentionBackend):
                             prompt_workgroups=self._prompt_workgroups(context, q.element_size()),
                             prompts_only=self._prompts_only(context, q.element_size()))
 
+    def decode_shared(self, q, k_cache, v_cache, context: Context, shared_len: int, out=None):
+        """``decode`` of rows whose first ``shared_len`` keys lie in the same pages (``shared_prefix_len`` finds how many),
+        those keys read once for all rows instead of once for each. q ``[B * Lq, Hq, D]``: each row's last ``Lq`` queries
+        (1, or drafts), row by row; ``context.context_lens`` counts all keys of a row, ``context.block_tables`` its whole
+        table. ``shared_len``: whole pages, those that row 0's table begins with. A row that is no longer than the shared
+        keys is attended by itself; one of no keys (graph padding) gets zeros. Nothing is read back, so a call can be
+        captured (a graph keeps ``shared_len``)."""
+        bt, lens = context.block_tables, context.context_lens
+        rows, page = lens.numel(), k_cache.size(1)
+        tokens, heads, dim = q.shape
+        cs = k_cache.stride()
+        if q.dtype not in _capi.DTYPES or heads != self.num_heads or dim != self.head_dim or q.stride(2) != 1:
+            raise ValueError(f"decode_shared: q is {q.dtype} {tuple(q.shape)} of strides {q.stride()}, not bf16 or fp16 "
+                             f"[T, {self.num_heads}, {self.head_dim}] of unit dim stride")
+        if (k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[2:] != (self.num_kv_heads, dim)
+                or cs != v_cache.stride() or cs[3] != 1 or not k_cache.dtype == v_cache.dtype == q.dtype):
+            raise ValueError(f"decode_shared: caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} of {k_cache.dtype}, "
+                             f"{v_cache.dtype}, strides {cs}, {v_cache.stride()}, for {self.num_kv_heads} kv heads of "
+                             f"{dim} in {q.dtype}")
+        if rows == 0 or tokens % rows:
+            raise ValueError(f"decode_shared: {tokens} queries do not divide over {rows} rows")
+        if bt.dtype != torch.int32 or bt.dim() != 2 or bt.size(0) != rows or (bt.size(1) > 1 and bt.stride(1) != 1):
+            raise ValueError(f"decode_shared: block tables {bt.dtype} {tuple(bt.shape)} for {rows} rows")
+        if shared_len < 0 or shared_len % page or shared_len > bt.size(1) * page:
+            raise ValueError(f"decode_shared: {shared_len} shared keys are not whole pages of {page} within tables of "
+                             f"{bt.size(1)} pages")
+        if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1):
+            raise ValueError(f"decode_shared: out is {out.dtype} {tuple(out.shape)}, not {q.dtype} {tuple(q.shape)}")
+        device = q.get_device()
+        if device < 0 or not all(t.get_device() == device for t in (k_cache, v_cache, bt, lens)
+                                 + (() if out is None else (out,))):
+            raise ValueError("decode_shared: all tensors must be on one GPU")
+        if lens.dtype != torch.int32 or not lens.is_contiguous():
+            lens = lens.to(torch.int32).contiguous()
+        if checks.ENABLED:
+            checks.check_tables(bt, k_cache.size(0))
+            checks.check_key_lengths(lens, bt, page)
+            checks.check_shared(bt, lens, shared_len // page, page, tokens // rows)
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        shape = (rows, tokens // rows, heads, self.num_kv_heads, dim)
+        max_k = bt.size(1) * page
+        # The partials are this call's own: calls on several streams, or graphs, share no workspace.
+        ws = torch.empty(_capi.query("lv_shared_prefix_workspace_bytes", *shape, page, shared_len, max_k) or 1,
+                         dtype=torch.uint8, device=q.device)
+        _capi.call_on(device, "lv_shared_prefix_decode", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
+                      v_cache.data_ptr(), cs[0], cs[1], cs[2], page, bt.data_ptr(), bt.stride(0), lens.data_ptr(), *shape,
+                      float(self.scale), shared_len, max_k, out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr(),
+                      ws.numel(), _capi.DTYPES[q.dtype])
+        return out
+
     def mla_decode(self, q, latent_cache, v_dim, context: Context, out=None):
         """Each row's last ``Lq`` queries against its paged latents, read as one key head shared by every query
         head; values are the latents' first ``v_dim`` entries (``abstract.py:206-219``). q ``[B * Lq, H, 576]``,

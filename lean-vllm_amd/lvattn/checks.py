@@ -79,6 +79,16 @@ def check_key_lengths(lens: torch.Tensor, block_tables: torch.Tensor, block_size
                          f" is -1")
 
 
+def check_shared(block_tables: torch.Tensor, lens: torch.Tensor, pages: int, block_size: int, queries: int) -> None:
+    """Every row that sees ``pages`` whole pages of keys from its first query on has row 0's first ``pages`` entries."""
+    t, lens = _host(block_tables), _host(lens).reshape(-1)
+    sees = lens - queries + 1 >= max(pages * block_size, 1)
+    bad = sees & (t[:, :pages] != t[0, :pages]).any(1)
+    if bad.any() or (sees.any() and (t[0, :pages] < 0).any()):
+        r = _first(bad) if bad.any() else 0
+        raise ValueError(f"row {r}'s first {pages} pages are not row 0's")
+
+
 def check_positions(positions: torch.Tensor, max_position: int) -> None:
     """Every position has a row in the rotary table (a padding row's negative one takes row 0)."""
     p = _host(positions).reshape(-1)
