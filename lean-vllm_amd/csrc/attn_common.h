@@ -123,10 +123,15 @@ __device__ __forceinline__ int swz(int r, int c) {
 // TP (paged keys, RING > 0): pages per 64-key tile -- 1 for pages of a multiple of 64 keys (one lookup per page,
 // kept across the page's tiles), 2 or 4 for pages of 32 or 16 keys (the tile's pages looked up at every fill, each
 // lane loading from its key's page).
+// PART (paged keys, RING > 0): an item that the caller has cut out by itself, whose partials another launch merges.
+struct PromptPart {
+  int lk, lq, tile0, tiles, slot0;  // `tiles` key tiles from tile0 on of lk keys, all seen by every one of lq queries from
+                                    // token 0 on; query j's partials go to slot slot0 + j of part_o / part_lse
+};
 template <typename T, int DQK, int DV, bool PREFETCH = true, bool OPAQUE_TID = false, int RING = 0, int WAVES = 4,
-          bool CTX = false, int TP = 1, bool SPLIT = false>
+          bool CTX = false, int TP = 1, bool SPLIT = false, bool PART = false>
 __device__ void prefill_item(const AttnParams& p, int row, int qtile, int kvh, char* smem, int piece = 0,
-                             int slot = 0) {
+                             int slot = 0, const PromptPart& part = {}) {
   using E = Elem<T>;
   constexpr int KS = DQK / 32;  // MFMA k-steps over the q.k width
   constexpr int DB = DV / 16;   // 16-dim blocks of the output
@@ -152,8 +157,9 @@ __device__ void prefill_item(const AttnParams& p, int row, int qtile, int kvh, c
   const int n = lane & 15, j4 = lane >> 4;
   const int G = p.group;
   const int qp = ROWS / G;  // positions per item
-  const int q0 = p.cu_q[row], lq = p.cu_q[row + 1] - q0;
-  const int lk = key_len(p, row);
+  static_assert(!PART || (RING > 0 && !CTX && !SPLIT), "cut-out items stream paged keys");
+  const int q0 = PART ? 0 : p.cu_q[row], lq = PART ? part.lq : p.cu_q[row + 1] - q0;
+  const int lk = PART ? part.lk : key_len(p, row);
   const int p0 = qtile * qp;
   if (p0 >= lq) return;  // a grid sized for the longest row
   const float c = p.scale_log2;
@@ -168,14 +174,14 @@ __device__ void prefill_item(const AttnParams& p, int row, int qtile, int kvh, c
     qi[nb] = p0 + mrow / G;
     head[nb] = kvh * G + mrow % G;
     qvalid[nb] = mrow < qp * G && qi[nb] < lq;
-    lim[nb] = qvalid[nb] && p.causal ? lk - lq + qi[nb] + 1 : lk;  // this query row sees keys < lim
+    lim[nb] = !PART && qvalid[nb] && p.causal ? lk - lq + qi[nb] + 1 : lk;  // this query row sees keys < lim
 #pragma unroll
     for (int k = 0; k < KS; ++k)
       qb[nb][k] = qvalid[nb] ? ld16(p.q + (int64_t)(q0 + qi[nb]) * p.q_st + head[nb] * p.q_sh +
                                     (int64_t)(32 * k + 8 * j4) * 2)
                              : u32x4{0, 0, 0, 0};
   }
-  const int kmax = p.causal ? min(lk, lk - lq + min(p0 + qp, lq)) : lk;  // keys the item needs
+  const int kmax = !PART && p.causal ? min(lk, lk - lq + min(p0 + qp, lq)) : lk;  // keys the item needs
   int lc = 0, cbase = 0;  // the row's context keys
   if constexpr (CTX) {
     cbase = p.cu_ctx[row];
@@ -185,8 +191,8 @@ __device__ void prefill_item(const AttnParams& p, int row, int qtile, int kvh, c
   const int all_tiles = nc + (kmax + kPrefillKeys - 1) / kPrefillKeys;    // all tiles of the item
   static_assert(!SPLIT || (RING > 0 && !CTX && WAVES == 4), "split items stream paged keys");
   const int per_piece = SPLIT ? (all_tiles + p.pieces - 1) / p.pieces : all_tiles;
-  const int tile0 = SPLIT ? min(piece * per_piece, all_tiles) : 0;
-  const int ntiles = SPLIT ? min(tile0 + per_piece, all_tiles) : all_tiles;  // this call's tiles: tile0 .. ntiles - 1
+  const int tile0 = PART ? part.tile0 : SPLIT ? min(piece * per_piece, all_tiles) : 0;
+  const int ntiles = PART ? part.tile0 + part.tiles : SPLIT ? min(tile0 + per_piece, all_tiles) : all_tiles;  // this call's tiles: tile0 .. ntiles - 1
 
   float m[2], l[2];  // raw-score max (held or running) and row sums
   f32x4 o[2][DB];
@@ -403,6 +409,10 @@ __device__ void prefill_item(const AttnParams& p, int row, int qtile, int kvh, c
         for (int q = 0; q < TP; ++q) pp[q] = table + min(t * TP + q, pg_last);
         int pg[TP];
         sload_n<TP>(pp, pg);
+        if constexpr (PART) {  // a step of padding rows has no shared pages: read anything
+#pragma unroll
+          for (int q = 0; q < TP; ++q) pg[q] = max(pg[q], 0);
+        }
 #pragma unroll
         for (int i = 0; i < (NJ + WAVES - 1) / WAVES; ++i) {
           const int j = wave + WAVES * i;
@@ -430,7 +440,8 @@ __device__ void prefill_item(const AttnParams& p, int row, int qtile, int kvh, c
         const int pg = (int)p.bs.div(kt);
         if (pg != cached_pg) {
           cached_pg = pg;
-          page_off = (int64_t)sload(table + pg) * p.c_sb;
+          const int page = sload(table + pg);
+          page_off = (int64_t)(PART ? max(page, 0) : page) * p.c_sb;
         }
         const int in_page = kt - pg * (int)p.bs.d;
         koff = page_off + (int64_t)in_page * p.c_st + kvh * p.c_sh;
@@ -528,6 +539,13 @@ __device__ void prefill_item(const AttnParams& p, int row, int qtile, int kvh, c
     const float lsum = xor32_sum(xor16_sum(l[nb]));
     if (!qvalid[nb]) continue;
     const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
+    if constexpr (PART) {  // as SPLIT's
+      const int64_t at = (int64_t)(part.slot0 + qi[nb]) * p.hq + head[nb];
+      if (j4 == 0) p.part_lse[at] = lsum > 0.f || lsum != lsum ? m[nb] * c + fast_log2(lsum) : -INFINITY;
+#pragma unroll
+      for (int b = 0; b < DB; ++b) *reinterpret_cast<f32x4*>(p.part_o + at * DV + b * 16 + 4 * j4) = o[nb][b] * inv;
+      continue;
+    }
     if constexpr (SPLIT) {
       const int64_t at = (int64_t)slot * kPrefillRows + wave * 32 + nb * 16 + n;
       // Of a NaN sum NaN, so that the merge keeps it where every piece's is one.

@@ -83,6 +83,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_prefix_kernel(SharedPar
   few_item<T, D, NB, SETS, true>(p, 0, 0, 0, kvh, smem, part);
 }
 
+// The prefix for more query rows than a few-query item holds: prompt items (attn_common.h), 128 rows against 64-key tiles
+// that the workgroup's waves share, two workgroups per CU. TP: pages per 64-key tile, as there.
+template <typename T, int D, int TP>
+__global__ __launch_bounds__(256, 2) void shared_tile_kernel(SharedParams p) {
+  __shared__ __attribute__((aligned(16))) char smem[2 * PromptSmem<D, D, (TP > 1)>::kBytes];
+  const int kvh = blockIdx.x % p.hkv, i = blockIdx.x / p.hkv;
+  const int piece = i / p.tiles, tile = i - piece * p.tiles;
+  PromptPart part;
+  part.lk = p.shared;
+  part.lq = p.tokens;
+  part.tile0 = piece * (p.per_piece / kPrefillKeys);
+  part.tiles = (min(p.per_piece, p.shared - piece * p.per_piece) + kPrefillKeys - 1) / kPrefillKeys;
+  part.slot0 = piece * p.tokens;
+  prefill_item<T, D, D, true, false, 2, 4, false, TP, false, true>(p, 0, tile, kvh, smem, 0, 0, part);
+}
+
 // One workgroup per (token, head): D / 4 threads a partial, 256 / (D / 4) partials at a time, joined through LDS.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void shared_merge_kernel(SharedParams p) {
@@ -148,6 +164,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedParams p) {
 
 // What the host decides from the shapes.
 struct SharedPlan {
+  int32_t tile_pages;  // pages per 64-key tile of prompt items (0: few-query items)
   int32_t tile_rows, tiles, pieces, per_piece, splits;
   size_t o_bytes, bytes;  // partial outputs, then their log-sum-exps
 };
@@ -155,12 +172,13 @@ struct SharedPlan {
 // (query, head) rows of a few-query item, by how many there are.
 static int few_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
-static SharedPlan shared_plan(int32_t rows, int32_t queries, int32_t hq, int32_t hkv, int32_t d, int32_t shared,
-                              int32_t max_k) {
+static SharedPlan shared_plan(int32_t rows, int32_t queries, int32_t hq, int32_t hkv, int32_t d, int32_t block_size,
+                              int32_t shared, int32_t max_k) {
   SharedPlan s{};
   const int group = hq / hkv;
   const int64_t tokens = (int64_t)rows * queries, query_rows = tokens * group;
-  s.tile_rows = few_rows(query_rows);
+  s.tile_pages = query_rows <= kFewMaxRows ? 0 : block_size % 64 == 0 ? 1 : block_size == 32 ? 2 : block_size == 16 ? 4 : 0;
+  s.tile_rows = s.tile_pages > 0 ? kPrefillRows / group * group : few_rows(query_rows);
   s.tiles = (int32_t)((query_rows + s.tile_rows - 1) / s.tile_rows);
   s.per_piece = 64;
   if (shared > 0) {
@@ -190,8 +208,15 @@ static void launch_few(const SharedParams& p, bool prefix, hipStream_t stream) {
 }
 
 template <typename T, int D>
-static int launch_shared(const SharedParams& p, hipStream_t stream) {
-  for (int prefix = p.pieces > 0; prefix >= 0; --prefix) {
+static int launch_shared(const SharedParams& p, int tile_pages, hipStream_t stream) {
+  if (tile_pages > 0 && p.pieces > 0) {
+    auto* const kernel = tile_pages == 1   ? &shared_tile_kernel<T, D, 1>
+                         : tile_pages == 2 ? &shared_tile_kernel<T, D, 2>
+                                           : &shared_tile_kernel<T, D, 4>;
+    hipLaunchKernelGGL(kernel, dim3(p.pieces * p.tiles * p.hkv), dim3(256), 0, stream, p);
+    LV_LAUNCH_CHECK("shared_tile_kernel");
+  }
+  for (int prefix = p.pieces > 0 && tile_pages == 0; prefix >= 0; --prefix) {
     const int rows = prefix ? p.tile_rows : few_rows(p.queries * p.group);
     if (rows <= 16) launch_few<T, D, 1, kOneSet>(p, prefix, stream);
     else if (rows <= 32) launch_few<T, D, 2, kOneSet>(p, prefix, stream);
@@ -236,7 +261,9 @@ extern "C" size_t lv_shared_prefix_workspace_bytes(int32_t num_rows, int32_t que
   if (num_rows <= 0 || check_shared(num_rows, queries_per_row, num_heads, num_kv_heads, head_dim, block_size,
                                     shared_len, max_seqlen_k) != LV_OK)
     return 0;
-  return shared_plan(num_rows, queries_per_row, num_heads, num_kv_heads, head_dim, shared_len, max_seqlen_k).bytes;
+  return shared_plan(num_rows, queries_per_row, num_heads, num_kv_heads, head_dim, block_size, shared_len,
+                     max_seqlen_k)
+      .bytes;
 }
 
 extern "C" int lv_shared_prefix_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
@@ -263,7 +290,7 @@ extern "C" int lv_shared_prefix_decode(const void* q, int64_t q_stride_t, int64_
              "shared_prefix_decode: cache token stride %lld is negative or too large", (long long)cache_stride_token);
   LV_REQUIRE(scale > 0.f, "shared_prefix_decode: the softmax scale must be positive, got %g", (double)scale);
   const SharedPlan s =
-      shared_plan(num_rows, queries_per_row, num_heads, num_kv_heads, head_dim, shared_len, max_seqlen_k);
+      shared_plan(num_rows, queries_per_row, num_heads, num_kv_heads, head_dim, block_size, shared_len, max_seqlen_k);
   LV_REQUIRE(workspace && workspace_bytes >= s.bytes, "shared_prefix_decode: workspace of %zu bytes given, %zu needed",
              workspace_bytes, s.bytes);
   LV_REQUIRE(aligned(workspace, 256), "shared_prefix_decode: workspace must be 256-byte aligned");
@@ -302,6 +329,6 @@ extern "C" int lv_shared_prefix_decode(const void* q, int64_t q_stride_t, int64_
   p.splits = s.splits;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (dtype == LV_DTYPE_BF16)
-    return head_dim == 64 ? launch_shared<BF16, 64>(p, st) : launch_shared<BF16, 128>(p, st);
-  return head_dim == 64 ? launch_shared<F16, 64>(p, st) : launch_shared<F16, 128>(p, st);
+    return head_dim == 64 ? launch_shared<BF16, 64>(p, s.tile_pages, st) : launch_shared<BF16, 128>(p, s.tile_pages, st);
+  return head_dim == 64 ? launch_shared<F16, 64>(p, s.tile_pages, st) : launch_shared<F16, 128>(p, s.tile_pages, st);
 }
