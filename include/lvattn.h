@@ -253,19 +253,21 @@ int lv_paged_attention_static(const void* q, int64_t q_stride_t, int64_t q_strid
  * q, out: [num_rows * queries_per_row, num_heads, head_dim], row b's queries consecutive; strides, caches, tables and
  * max_seqlen_k as lv_paged_attention's. head_dim 64 or 128; queries_per_row times query heads per kv head at most 64;
  * pages of a multiple of 16.
+ * own_keys: about how many keys the rows have behind the shared ones in all, or 0 where the host does not know; it only
+ * sizes the work.
  * workspace: at least lv_shared_prefix_workspace_bytes(...) bytes for the same arguments, 256-byte aligned; no
  * initialisation needed and nothing kept in it, but it must not be one that holds a step's plan
  * (LV_ATTN_REUSE_PLAN). */
 size_t lv_shared_prefix_workspace_bytes(int32_t num_rows, int32_t queries_per_row, int32_t num_heads,
                                         int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t shared_len,
-                                        int32_t max_seqlen_k);
+                                        int32_t max_seqlen_k, int64_t own_keys);
 int lv_shared_prefix_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
                             const void* v_cache, int64_t cache_stride_block, int64_t cache_stride_token,
                             int64_t cache_stride_head, int32_t block_size, const int32_t* block_tables,
                             int64_t table_stride, const int32_t* context_lens, int32_t num_rows,
                             int32_t queries_per_row, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                            float scale, int32_t shared_len, int32_t max_seqlen_k, void* out, int64_t out_stride_t,
-                            int64_t out_stride_h, void* workspace, size_t workspace_bytes, int32_t dtype,
+                            float scale, int32_t shared_len, int32_t max_seqlen_k, int64_t own_keys, void* out,
+                            int64_t out_stride_t, int64_t out_stride_h, void* workspace, size_t workspace_bytes, int32_t dtype,
                             void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------

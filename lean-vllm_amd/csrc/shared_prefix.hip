@@ -17,7 +17,8 @@ constexpr int kSharedRound = 512;    // workgroups that run at once (two per CU)
 constexpr int kOwnKeys = 256;        // least keys a row's own split is cut for
 constexpr int kSharedPieceKeys = 256;  // and a piece of the prefix
 constexpr int kMaxOwnSplits = 32;
-constexpr int kMaxSharedPieces = 64;
+constexpr int kMaxSharedPieces = 256;
+constexpr double kTilesPerUs = 245, kTileUs = 1.32, kOwnBytesPerUs = 6.0e6;
 
 struct SharedParams : AttnParams {
   int32_t shared, queries, tokens;  // keys of the prefix; queries per row; all queries
@@ -42,10 +43,64 @@ __device__ __forceinline__ OwnSpan own_span(const SharedParams& p, int len) {
 
 // Partials lie by slot: piece i of token t's prefix in slot i tokens + t, its row's own split j in slot
 // (pieces + j) tokens + t.
-template <typename T, int D, int NB, FewSets SETS>
-__global__ __launch_bounds__(64 * kWaves, 2) void shared_own_kernel(SharedParams p) {
-  __shared__ __attribute__((aligned(16))) char smem[kWaves * kFewStages * kFewStage];
-  const int kvh = blockIdx.x % p.hkv, i = blockIdx.x / p.hkv;
+
+// How a kernel computes its items. Few<ROWS>: few-query items (few_item.h) of at most 16, 32 or 64 (query, head) rows, of
+// the prefix or of a row's own keys. Tile<TP>: prompt items (attn_common.h), 128 rows of the prefix against 64-key tiles
+// that the workgroup's waves share; TP: pages per 64-key tile, as there.
+template <int ROWS, int HP = 1>
+struct Few {
+  template <int D>
+  static constexpr int bytes() { return kWaves * kFewStages * kFewStage; }
+  template <typename T, int D>
+  static __device__ __forceinline__ void attend(const SharedParams& p, int kvh, char* smem, const FewPart& part) {
+    constexpr bool two = ROWS == 64 && D == 128;  // as few_query.hip's launches
+    few_item<T, D, (two ? 2 : ROWS / 16), (HP == 2 ? kTwoHeads : two ? kTwoBlocks : kOneSet), true>(p, 0, 0, 0, kvh, smem, part);
+  }
+  template <typename T, int D>
+  static __device__ __forceinline__ void prefix(const SharedParams& p, int kvh, int piece, int tile, char* smem) {
+    FewPart part;
+    part.table = p.tables;
+    part.lk = p.shared;
+    part.lq = p.tokens;
+    part.tok = 0;
+    part.kbeg = piece * p.per_piece;
+    part.kend = min(p.shared, part.kbeg + p.per_piece);
+    part.row0 = tile * p.tile_rows;
+    part.row_end = min(p.tokens * p.group, part.row0 + p.tile_rows);
+    part.slot0 = piece * p.tokens;
+    part.causal = false;
+    attend<T, D>(p, kvh, smem, part);
+  }
+};
+template <int TP>
+struct Tile {
+  template <int D>
+  static constexpr int bytes() { return 2 * PromptSmem<D, D, (TP > 1)>::kBytes; }
+  template <typename T, int D>
+  static __device__ __forceinline__ void prefix(const SharedParams& p, int kvh, int piece, int tile, char* smem) {
+    PromptPart part;
+    part.lk = p.shared;
+    part.lq = p.tokens;
+    part.tile0 = piece * (p.per_piece / kPrefillKeys);
+    part.tiles = (min(p.per_piece, p.shared - piece * p.per_piece) + kPrefillKeys - 1) / kPrefillKeys;
+    part.slot0 = piece * p.tokens;
+    prefill_item<T, D, D, true, false, 2, 4, false, TP, false, true>(p, 0, tile, kvh, smem, 0, 0, part);
+  }
+};
+// Workgroups [0, prefix_wgs) take the prefix's items, the rest the rows' own.
+template <typename T, int D, typename PREFIX, int OWN_ROWS, int HP>
+__global__ __launch_bounds__(256, 2) void shared_items_kernel(SharedParams p, int32_t prefix_wgs) {
+  constexpr int kBytes = std::max(PREFIX::template bytes<D>(), Few<OWN_ROWS, HP>::template bytes<D>());
+  __shared__ __attribute__((aligned(16))) char smem[kBytes];
+  int b = blockIdx.x;
+  if (b < prefix_wgs) {
+    const int kvh = b % p.hkv, i = b / p.hkv;
+    const int piece = i / p.tiles, tile = i - piece * p.tiles;
+    PREFIX::template prefix<T, D>(p, kvh, piece, tile, smem);
+    return;
+  }
+  b -= prefix_wgs;
+  const int ny = p.hkv / HP, kvh = b % ny * HP, i = b / ny;
   const int split = i / p.rows, row = i - split * p.rows;
   const int len = sload(p.lens_k + row);
   const OwnSpan s = own_span(p, len);
@@ -61,42 +116,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_own_kernel(SharedParams
   part.row_end = p.queries * p.group;
   part.slot0 = (p.pieces + split) * p.tokens + part.tok;
   part.causal = true;
-  few_item<T, D, NB, SETS, true>(p, row, 0, 0, kvh, smem, part);
-}
-
-template <typename T, int D, int NB, FewSets SETS>
-__global__ __launch_bounds__(64 * kWaves, 2) void shared_prefix_kernel(SharedParams p) {
-  __shared__ __attribute__((aligned(16))) char smem[kWaves * kFewStages * kFewStage];
-  const int kvh = blockIdx.x % p.hkv, i = blockIdx.x / p.hkv;
-  const int piece = i / p.tiles, tile = i - piece * p.tiles;
-  FewPart part;
-  part.table = p.tables;
-  part.lk = p.shared;
-  part.lq = p.tokens;
-  part.tok = 0;
-  part.kbeg = piece * p.per_piece;
-  part.kend = min(p.shared, part.kbeg + p.per_piece);
-  part.row0 = tile * p.tile_rows;
-  part.row_end = min(p.tokens * p.group, part.row0 + p.tile_rows);
-  part.slot0 = piece * p.tokens;
-  part.causal = false;
-  few_item<T, D, NB, SETS, true>(p, 0, 0, 0, kvh, smem, part);
-}
-
-// The prefix for more query rows than a few-query item holds: prompt items (attn_common.h), 128 rows against 64-key tiles
-// that the workgroup's waves share, two workgroups per CU. TP: pages per 64-key tile, as there.
-template <typename T, int D, int TP>
-__global__ __launch_bounds__(256, 2) void shared_tile_kernel(SharedParams p) {
-  __shared__ __attribute__((aligned(16))) char smem[2 * PromptSmem<D, D, (TP > 1)>::kBytes];
-  const int kvh = blockIdx.x % p.hkv, i = blockIdx.x / p.hkv;
-  const int piece = i / p.tiles, tile = i - piece * p.tiles;
-  PromptPart part;
-  part.lk = p.shared;
-  part.lq = p.tokens;
-  part.tile0 = piece * (p.per_piece / kPrefillKeys);
-  part.tiles = (min(p.per_piece, p.shared - piece * p.per_piece) + kPrefillKeys - 1) / kPrefillKeys;
-  part.slot0 = piece * p.tokens;
-  prefill_item<T, D, D, true, false, 2, 4, false, TP, false, true>(p, 0, tile, kvh, smem, 0, 0, part);
+  Few<OWN_ROWS, HP>::template attend<T, D>(p, kvh, smem, part);
 }
 
 // One workgroup per (token, head): D / 4 threads a partial, 256 / (D / 4) partials at a time, joined through LDS.
@@ -165,7 +185,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedParams p) {
 // What the host decides from the shapes.
 struct SharedPlan {
   int32_t tile_pages;  // pages per 64-key tile of prompt items (0: few-query items)
-  int32_t tile_rows, tiles, pieces, per_piece, splits;
+  int32_t tile_rows, tiles, pieces, per_piece, splits, own_heads;
   size_t o_bytes, bytes;  // partial outputs, then their log-sum-exps
 };
 
@@ -173,56 +193,62 @@ struct SharedPlan {
 static int few_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
 static SharedPlan shared_plan(int32_t rows, int32_t queries, int32_t hq, int32_t hkv, int32_t d, int32_t block_size,
-                              int32_t shared, int32_t max_k) {
+                              int32_t shared, int32_t max_k, int64_t own_keys) {
   SharedPlan s{};
   const int group = hq / hkv;
   const int64_t tokens = (int64_t)rows * queries, query_rows = tokens * group;
-  s.tile_pages = query_rows <= kFewMaxRows ? 0 : block_size % 64 == 0 ? 1 : block_size == 32 ? 2 : block_size == 16 ? 4 : 0;
+  if (query_rows > (d == 64 ? 64 : 32))
+    s.tile_pages = block_size % 64 == 0 ? 1 : block_size == 32 ? 2 : block_size == 16 ? 4 : 0;
   s.tile_rows = s.tile_pages > 0 ? kPrefillRows / group * group : few_rows(query_rows);
   s.tiles = (int32_t)((query_rows + s.tile_rows - 1) / s.tile_rows);
-  s.per_piece = 64;
+  // Unknown: half the bound; for the prefix's pieces, which a bound far off would make too few, at most 1024 a row.
+  const int64_t row_keys = own_keys > 0 ? own_keys / rows : (max_k - shared) / 2;
+  if (own_keys <= 0) own_keys = (int64_t)rows * std::min<int64_t>(row_keys + 1, 1024);
+  const double own_us = (double)own_keys * hkv * d * 4 / kOwnBytesPerUs;
+  s.per_piece = kPrefillKeys;
   if (shared > 0) {
-    const int64_t units = (int64_t)s.tiles * hkv;
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>({kSharedRound / units, kMaxSharedPieces,
-                                                                 shared / kSharedPieceKeys}));
+    const int64_t units = (int64_t)s.tiles * hkv, key_tiles = (shared + kPrefillKeys - 1) / kPrefillKeys;
+    const bool beside = s.tile_pages == 0 || own_us > 0.3 * (double)(units * key_tiles) / kTilesPerUs;
+    int64_t want = (beside ? kSharedRound / 2 : kSharedRound) / units;
+    if (s.tile_pages > 0 && beside)
+      want = std::min(want, (int64_t)std::ceil((double)key_tiles * kTileUs / std::max(0.75 * own_us, 8.0)));
+    want = std::max<int64_t>(1, std::min<int64_t>({want, kMaxSharedPieces, shared / kSharedPieceKeys}));
     s.per_piece = (int32_t)(((shared + want - 1) / want + 63) / 64 * 64);
     s.pieces = (shared + s.per_piece - 1) / s.per_piece;
   }
+  s.own_heads = hkv % 2 == 0 && (int64_t)rows * hkv >= kSharedRound / 2 && queries * group <= 32 ? 2 : 1;
+  const int64_t units = (int64_t)rows * hkv / s.own_heads, half = kSharedRound / 2;
+  int64_t splits = units <= half ? half / units : 2;
+  splits = std::max(splits, std::min<int64_t>((4 * kSharedRound + units - 1) / units, row_keys / 1024));
   // A row that does not see the prefix walks all its keys, so the bound is on those, not on the keys behind it.
-  const int64_t units = (int64_t)rows * hkv;
-  s.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({(kSharedRound + units - 1) / units, kMaxOwnSplits,
-                                                              ((int64_t)max_k + kOwnKeys - 1) / kOwnKeys}));
+  s.splits = (int32_t)std::max<int64_t>(
+      1, std::min<int64_t>({splits, kMaxOwnSplits, ((int64_t)max_k + kOwnKeys - 1) / kOwnKeys}));
   const int64_t partials = ((int64_t)s.pieces + s.splits) * tokens * hq;
   s.o_bytes = (size_t)partials * d * sizeof(float);
   s.bytes = s.o_bytes + (size_t)partials * sizeof(float);
   return s;
 }
 
-template <typename T, int D, int NB, FewSets SETS>
-static void launch_few(const SharedParams& p, bool prefix, hipStream_t stream) {
-  const dim3 block(64 * kWaves);
-  if (prefix)
-    hipLaunchKernelGGL((shared_prefix_kernel<T, D, NB, SETS>), dim3(p.pieces * p.tiles * p.hkv), block, 0, stream, p);
-  else
-    hipLaunchKernelGGL((shared_own_kernel<T, D, NB, SETS>), dim3(p.splits * p.rows * p.hkv), block, 0, stream, p);
+template <typename T, int D, typename PREFIX>
+static void launch_items(const SharedParams& p, int own_heads, hipStream_t stream) {
+  const int rows = p.queries * p.group, prefix = p.pieces * p.tiles * p.hkv;
+  auto* const kernel = rows <= 16   ? (own_heads == 2 ? &shared_items_kernel<T, D, PREFIX, 16, 2>
+                                                      : &shared_items_kernel<T, D, PREFIX, 16, 1>)
+                       : rows <= 32 ? (own_heads == 2 ? &shared_items_kernel<T, D, PREFIX, 32, 2>
+                                                      : &shared_items_kernel<T, D, PREFIX, 32, 1>)
+                                    : &shared_items_kernel<T, D, PREFIX, 64, 1>;
+  hipLaunchKernelGGL(kernel, dim3(prefix + p.splits * p.rows * (p.hkv / own_heads)), dim3(256), 0, stream, p, prefix);
 }
 
 template <typename T, int D>
-static int launch_shared(const SharedParams& p, int tile_pages, hipStream_t stream) {
-  if (tile_pages > 0 && p.pieces > 0) {
-    auto* const kernel = tile_pages == 1   ? &shared_tile_kernel<T, D, 1>
-                         : tile_pages == 2 ? &shared_tile_kernel<T, D, 2>
-                                           : &shared_tile_kernel<T, D, 4>;
-    hipLaunchKernelGGL(kernel, dim3(p.pieces * p.tiles * p.hkv), dim3(256), 0, stream, p);
-    LV_LAUNCH_CHECK("shared_tile_kernel");
-  }
-  for (int prefix = p.pieces > 0 && tile_pages == 0; prefix >= 0; --prefix) {
-    const int rows = prefix ? p.tile_rows : few_rows(p.queries * p.group);
-    if (rows <= 16) launch_few<T, D, 1, kOneSet>(p, prefix, stream);
-    else if (rows <= 32) launch_few<T, D, 2, kOneSet>(p, prefix, stream);
-    else launch_few<T, D, (D == 64 ? 4 : 2), (D == 64 ? kOneSet : kTwoBlocks)>(p, prefix, stream);
-    LV_LAUNCH_CHECK("shared-prefix attention kernel");
-  }
+static int launch_shared(const SharedParams& p, const SharedPlan& s, hipStream_t stream) {
+  if (s.tile_pages == 1) launch_items<T, D, Tile<1>>(p, s.own_heads, stream);
+  else if (s.tile_pages == 2) launch_items<T, D, Tile<2>>(p, s.own_heads, stream);
+  else if (s.tile_pages == 4) launch_items<T, D, Tile<4>>(p, s.own_heads, stream);
+  else if (p.tile_rows == 16) launch_items<T, D, Few<16>>(p, s.own_heads, stream);
+  else if (p.tile_rows == 32) launch_items<T, D, Few<32>>(p, s.own_heads, stream);
+  else launch_items<T, D, Few<64>>(p, s.own_heads, stream);
+  LV_LAUNCH_CHECK("shared_items_kernel");
   hipLaunchKernelGGL((shared_merge_kernel<T, D>), dim3(p.tokens * p.hq), dim3(256), 0, stream, p);
   LV_LAUNCH_CHECK("shared_merge_kernel");
   return LV_OK;
@@ -257,12 +283,12 @@ using namespace lv;
 
 extern "C" size_t lv_shared_prefix_workspace_bytes(int32_t num_rows, int32_t queries_per_row, int32_t num_heads,
                                                    int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
-                                                   int32_t shared_len, int32_t max_seqlen_k) {
+                                                   int32_t shared_len, int32_t max_seqlen_k, int64_t own_keys) {
   if (num_rows <= 0 || check_shared(num_rows, queries_per_row, num_heads, num_kv_heads, head_dim, block_size,
                                     shared_len, max_seqlen_k) != LV_OK)
     return 0;
   return shared_plan(num_rows, queries_per_row, num_heads, num_kv_heads, head_dim, block_size, shared_len,
-                     max_seqlen_k)
+                     max_seqlen_k, own_keys)
       .bytes;
 }
 
@@ -272,7 +298,7 @@ extern "C" int lv_shared_prefix_decode(const void* q, int64_t q_stride_t, int64_
                                        int64_t table_stride, const int32_t* context_lens, int32_t num_rows,
                                        int32_t queries_per_row, int32_t num_heads, int32_t num_kv_heads,
                                        int32_t head_dim, float scale, int32_t shared_len, int32_t max_seqlen_k,
-                                       void* out, int64_t out_stride_t, int64_t out_stride_h, void* workspace,
+                                       int64_t own_keys, void* out, int64_t out_stride_t, int64_t out_stride_h, void* workspace,
                                        size_t workspace_bytes, int32_t dtype, void* stream) {
   LV_REQUIRE(dtype == LV_DTYPE_BF16 || dtype == LV_DTYPE_F16, "shared_prefix_decode: dtype %d is not bf16 or fp16",
              dtype);
@@ -290,7 +316,8 @@ extern "C" int lv_shared_prefix_decode(const void* q, int64_t q_stride_t, int64_
              "shared_prefix_decode: cache token stride %lld is negative or too large", (long long)cache_stride_token);
   LV_REQUIRE(scale > 0.f, "shared_prefix_decode: the softmax scale must be positive, got %g", (double)scale);
   const SharedPlan s =
-      shared_plan(num_rows, queries_per_row, num_heads, num_kv_heads, head_dim, block_size, shared_len, max_seqlen_k);
+      shared_plan(num_rows, queries_per_row, num_heads, num_kv_heads, head_dim, block_size, shared_len, max_seqlen_k,
+                  own_keys);
   LV_REQUIRE(workspace && workspace_bytes >= s.bytes, "shared_prefix_decode: workspace of %zu bytes given, %zu needed",
              workspace_bytes, s.bytes);
   LV_REQUIRE(aligned(workspace, 256), "shared_prefix_decode: workspace must be 256-byte aligned");
@@ -329,6 +356,6 @@ extern "C" int lv_shared_prefix_decode(const void* q, int64_t q_stride_t, int64_
   p.splits = s.splits;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (dtype == LV_DTYPE_BF16)
-    return head_dim == 64 ? launch_shared<BF16, 64>(p, s.tile_pages, st) : launch_shared<BF16, 128>(p, s.tile_pages, st);
-  return head_dim == 64 ? launch_shared<F16, 64>(p, s.tile_pages, st) : launch_shared<F16, 128>(p, s.tile_pages, st);
+    return head_dim == 64 ? launch_shared<BF16, 64>(p, s, st) : launch_shared<BF16, 128>(p, s, st);
+  return head_dim == 64 ? launch_shared<F16, 64>(p, s, st) : launch_shared<F16, 128>(p, s, st);
 }

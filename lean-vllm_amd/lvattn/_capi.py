@@ -45,10 +45,11 @@ _PROTOTYPES = {
                                                  _P, c_int64, _P, _P, _P, c_int32, c_int32, c_int32, c_int32,
                                                  c_int32, c_float, c_int32, c_int32, _P, c_int64, c_int64, c_int32,
                                                  c_int32, c_int32, c_int32, _P]),
-    "lv_shared_prefix_workspace_bytes": (c_size_t, [c_int32] * 8),
+    "lv_shared_prefix_workspace_bytes": (c_size_t, [c_int32] * 8 + [c_int64]),
     "lv_shared_prefix_decode": (ctypes.c_int, [_P, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int32, _P,
                                                c_int64, _P, c_int32, c_int32, c_int32, c_int32, c_int32, c_float,
-                                               c_int32, c_int32, _P, c_int64, c_int64, _P, c_size_t, c_int32, _P]),
+                                               c_int32, c_int32, c_int64, _P, c_int64, c_int64, _P, c_size_t, c_int32,
+                                               _P]),
     "lv_merge_attn_states": (ctypes.c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64,
                                             _P, c_int64, c_int64, _P, c_int64, c_int64, c_int32, c_int32,
                                             c_int32, c_int32, _P]),

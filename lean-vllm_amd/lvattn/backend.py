@@ -365,12 +365,14 @@ class MI355XAttention(AttentionBackend):
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         shape = (rows, tokens // rows, heads, self.num_kv_heads, dim)
         max_k = bt.size(1) * page
+        cu_k = context.cu_seqlens_k_host
+        own_keys = 0 if cu_k is None else max(cu_k[-1] - rows * shared_len, 0)
         # The partials are this call's own: calls on several streams, or graphs, share no workspace.
-        ws = torch.empty(_capi.query("lv_shared_prefix_workspace_bytes", *shape, page, shared_len, max_k) or 1,
+        ws = torch.empty(_capi.query("lv_shared_prefix_workspace_bytes", *shape, page, shared_len, max_k, own_keys) or 1,
                          dtype=torch.uint8, device=q.device)
         _capi.call_on(device, "lv_shared_prefix_decode", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
                       v_cache.data_ptr(), cs[0], cs[1], cs[2], page, bt.data_ptr(), bt.stride(0), lens.data_ptr(), *shape,
-                      float(self.scale), shared_len, max_k, out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr(),
+                      float(self.scale), shared_len, max_k, own_keys, out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr(),
                       ws.numel(), _capi.DTYPES[q.dtype])
         return out
 

@@ -72,7 +72,7 @@ def test_the_debug_check_finds_pages_that_are_not_shared():
 def c_call(*, rows=4, queries=1, hq=8, hk=2, dim=64, page=16, shared=32, max_k=96, scale=0.1, ws=16, nbytes=1 << 40,
            dtype=0, q=16, stride=64):
     _capi.call("lv_shared_prefix_decode", q, 8 * 64, stride, 16, 16, 2048, 128, 64, page, 16, 6, 16, rows, queries, hq, hk,
-               dim, scale, shared, max_k, 16, 512, 64, ws, nbytes, dtype, None)
+               dim, scale, shared, max_k, 0, 16, 512, 64, ws, nbytes, dtype, None)
 
 
 @pytest.mark.parametrize("change,message", [
@@ -92,8 +92,8 @@ def test_the_c_entry_refuses(change, message):
 def test_no_rows_and_the_workspace():
     c_call(rows=0)
 
-    def size(*a):
-        return _capi.query("lv_shared_prefix_workspace_bytes", *a)
+    def size(*a, own_keys=0):
+        return _capi.query("lv_shared_prefix_workspace_bytes", *a, own_keys)
 
     assert size(0, 1, 8, 2, 64, 16, 32, 96) == 0 and size(4, 1, 8, 3, 64, 16, 32, 96) == 0
     assert 0 < size(4, 1, 16, 8, 128, 16, 2048, 4096) < 8 << 20
