@@ -330,50 +330,51 @@ class MI355XAttention(AttentionBackend):
         table. ``shared_len``: whole pages, those that row 0's table begins with. A row that is no longer than the shared
         keys is attended by itself; one of no keys (graph padding) gets zeros. Nothing is read back, so a call can be
         captured (a graph keeps ``shared_len``)."""
+        what = "decode_shared"
         bt, lens = context.block_tables, context.context_lens
-        rows, page = lens.numel(), k_cache.size(1)
         tokens, heads, dim = q.shape
-        cs = k_cache.stride()
-        if q.dtype not in _capi.DTYPES or heads != self.num_heads or dim != self.head_dim or q.stride(2) != 1:
-            raise ValueError(f"decode_shared: q is {q.dtype} {tuple(q.shape)} of strides {q.stride()}, not bf16 or fp16 "
+        kv_heads, dtype, device, qs = self.num_kv_heads, q.dtype, q.get_device(), q.stride()
+        shape, cs = k_cache.shape, k_cache.stride()
+        rows, width = bt.shape
+        page = shape[1]
+        if dtype not in _capi.DTYPES or heads != self.num_heads or dim != self.head_dim or qs[2] != 1:
+            raise ValueError(f"{what}: q is {dtype} {tuple(q.shape)} of strides {qs}, not bf16 or fp16 "
                              f"[T, {self.num_heads}, {self.head_dim}] of unit dim stride")
-        if (k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[2:] != (self.num_kv_heads, dim)
-                or cs != v_cache.stride() or cs[3] != 1 or not k_cache.dtype == v_cache.dtype == q.dtype):
-            raise ValueError(f"decode_shared: caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} of {k_cache.dtype}, "
-                             f"{v_cache.dtype}, strides {cs}, {v_cache.stride()}, for {self.num_kv_heads} kv heads of "
-                             f"{dim} in {q.dtype}")
+        if (len(shape) != 4 or shape[2] != kv_heads or shape[3] != dim or shape != v_cache.shape or cs[3] != 1
+                or cs != v_cache.stride() or not k_cache.dtype is v_cache.dtype is dtype):
+            raise ValueError(f"{what}: caches {tuple(shape)} and {tuple(v_cache.shape)} of {k_cache.dtype}, "
+                             f"{v_cache.dtype}, strides {cs}, {v_cache.stride()}, for {kv_heads} kv heads of {dim} in "
+                             f"{dtype}")
+        if bt.dtype is not torch.int32 or lens.shape != (rows,) or (width > 1 and bt.stride(1) != 1):
+            raise ValueError(f"{what}: block tables {bt.dtype} {tuple(bt.shape)} for {lens.numel()} rows")
         if rows == 0 or tokens % rows:
-            raise ValueError(f"decode_shared: {tokens} queries do not divide over {rows} rows")
-        if bt.dtype != torch.int32 or bt.dim() != 2 or bt.size(0) != rows or (bt.size(1) > 1 and bt.stride(1) != 1):
-            raise ValueError(f"decode_shared: block tables {bt.dtype} {tuple(bt.shape)} for {rows} rows")
-        if shared_len < 0 or shared_len % page or shared_len > bt.size(1) * page:
-            raise ValueError(f"decode_shared: {shared_len} shared keys are not whole pages of {page} within tables of "
-                             f"{bt.size(1)} pages")
-        if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1):
-            raise ValueError(f"decode_shared: out is {out.dtype} {tuple(out.shape)}, not {q.dtype} {tuple(q.shape)}")
-        device = q.get_device()
-        if device < 0 or not all(t.get_device() == device for t in (k_cache, v_cache, bt, lens)
-                                 + (() if out is None else (out,))):
-            raise ValueError("decode_shared: all tensors must be on one GPU")
-        if lens.dtype != torch.int32 or not lens.is_contiguous():
-            lens = lens.to(torch.int32).contiguous()
-        if checks.ENABLED:
-            checks.check_tables(bt, k_cache.size(0))
-            checks.check_key_lengths(lens, bt, page)
-            checks.check_shared(bt, lens, shared_len // page, page, tokens // rows)
+            raise ValueError(f"{what}: {tokens} queries do not divide over {rows} rows")
+        if shared_len < 0 or shared_len % page or shared_len > width * page:
+            raise ValueError(f"{what}: {shared_len} shared keys are not whole pages of {page} within tables of {width} "
+                             "pages")
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        shape = (rows, tokens // rows, heads, self.num_kv_heads, dim)
-        max_k = bt.size(1) * page
-        cu_k = context.cu_seqlens_k_host
+        elif out.shape != q.shape or out.dtype is not dtype or out.stride(2) != 1 or out.get_device() != device:
+            raise ValueError(f"{what}: out is {out.dtype} {tuple(out.shape)}, not {dtype} {tuple(q.shape)} beside q")
+        if device < 0 or not (k_cache.get_device() == v_cache.get_device() == bt.get_device() == lens.get_device()
+                              == device):
+            raise ValueError(f"{what}: all tensors must be on one GPU")
+        if lens.dtype is not torch.int32 or not lens.is_contiguous():
+            lens = lens.to(torch.int32).contiguous()
+        if checks.ENABLED:
+            checks.check_tables(bt, shape[0])
+            checks.check_key_lengths(lens, bt, page)
+            checks.check_shared(bt, lens, shared_len // page, page, tokens // rows)
+        sizes = (rows, tokens // rows, heads, kv_heads, dim)
+        max_k, cu_k, os_ = width * page, context.cu_seqlens_k_host, out.stride()
         own_keys = 0 if cu_k is None else max(cu_k[-1] - rows * shared_len, 0)
         # The partials are this call's own: calls on several streams, or graphs, share no workspace.
-        ws = torch.empty(_capi.query("lv_shared_prefix_workspace_bytes", *shape, page, shared_len, max_k, own_keys) or 1,
-                         dtype=torch.uint8, device=q.device)
-        _capi.call_on(device, "lv_shared_prefix_decode", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
-                      v_cache.data_ptr(), cs[0], cs[1], cs[2], page, bt.data_ptr(), bt.stride(0), lens.data_ptr(), *shape,
-                      float(self.scale), shared_len, max_k, own_keys, out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr(),
-                      ws.numel(), _capi.DTYPES[q.dtype])
+        nbytes = _capi.query("lv_shared_prefix_workspace_bytes", *sizes, page, shared_len, max_k, own_keys) or 1
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        _capi.call_on(device, "lv_shared_prefix_decode", q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(),
+                      v_cache.data_ptr(), cs[0], cs[1], cs[2], page, bt.data_ptr(), bt.stride(0), lens.data_ptr(), *sizes,
+                      self.scale, shared_len, max_k, own_keys, out.data_ptr(), os_[0], os_[1], ws.data_ptr(), nbytes,
+                      _capi.DTYPES[dtype])
         return out
 
     def mla_decode(self, q, latent_cache, v_dim, context: Context, out=None):
