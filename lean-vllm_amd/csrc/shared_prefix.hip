@@ -6,18 +6,34 @@
 // shared ranges can be walked with every row's queries together: their keys are read rows times less often than by
 // lv_paged_attention (math of TorchAttention.decode, lean_vllm/attention/torch_backend.py:93-103, row by row).
 //
-// Three launches: the prefix (query tiles x kv heads x pieces of its keys), the rows' own keys (rows x kv heads x splits),
-// and the merge of the fp32 partials. Everything is sized by the host from shapes and bounds; the rows' lengths are read
-// on the device, so a call can be captured.
+// Two launches: the items, which are the prefix's (query tiles x kv heads x pieces of its keys) and the rows' own (rows x
+// kv heads x splits of their keys), and the merge of their fp32 partials. Everything is sized by the host from shapes and
+// bounds; the rows' lengths are read on the device, so a call can be captured.
+//
+// What bounds it: the prefix's items MFMA once some 100 query rows share a kv head, the rows' own and small batches HBM.
+// The two kinds run in one launch, the prefix's first, on a grid that gives them one of the two workgroups that a CU holds
+// and the rows' own the other, so that one kind's MFMA work runs under the other's loads. Measured, 32/8 heads, d128, bf16
+// (prefix keys, rows, own keys a row; us):
+//                                         one launch      prefix, own and merge launches   lv_paged_attention
+//   32,768, 200 rows, 64-2048             231             303                              2380
+//   8192, 64 rows, 16-1024                46.8            60.8                             244
+//   2048, 128 rows, 64-1024, 16 a page    64.6            80.4                             149
+//   65,536, 256 rows, 16-64               287             312                              5786
+//   16,384, 16 rows, 64-512               24.9            38.6                             123
+// What is left at 200 rows: the prefix alone takes 134 us on whole CUs and 179 on one workgroup of each, the own keys alone
+// 161 (4 to 9 pieces of the prefix 231 / 240 / 252 / 264 / - / 281 us; raised wave priority of either kind 232 and 269;
+// partials stored past the caches 231; a last tile's empty waves that skip the products 232).
 #include "few_item.h"
 
 namespace lv {
 
-constexpr int kSharedRound = 512;    // workgroups that run at once (two per CU)
-constexpr int kOwnKeys = 256;        // least keys a row's own split is cut for
+constexpr int kSharedRound = 512;      // workgroups that run at once (two per CU)
+constexpr int kOwnKeys = 256;          // least keys a row's own split is cut for
 constexpr int kSharedPieceKeys = 256;  // and a piece of the prefix
 constexpr int kMaxOwnSplits = 32;
 constexpr int kMaxSharedPieces = 256;
+// 64-key tiles of prompt items that the GPU takes in a microsecond with two workgroups on each CU (245; 190 with one), and
+// one such workgroup's time for a tile; the rate at which own keys stream. 32/8 heads of 128 and 64/8 of 64.
 constexpr double kTilesPerUs = 245, kTileUs = 1.32, kOwnBytesPerUs = 6.0e6;
 
 struct SharedParams : AttnParams {
@@ -49,12 +65,14 @@ __device__ __forceinline__ OwnSpan own_span(const SharedParams& p, int len) {
 // that the workgroup's waves share; TP: pages per 64-key tile, as there.
 template <int ROWS, int HP = 1>
 struct Few {
+  static constexpr int kRows = ROWS;
   template <int D>
   static constexpr int bytes() { return kWaves * kFewStages * kFewStage; }
   template <typename T, int D>
   static __device__ __forceinline__ void attend(const SharedParams& p, int kvh, char* smem, const FewPart& part) {
     constexpr bool two = ROWS == 64 && D == 128;  // as few_query.hip's launches
-    few_item<T, D, (two ? 2 : ROWS / 16), (HP == 2 ? kTwoHeads : two ? kTwoBlocks : kOneSet), true>(p, 0, 0, 0, kvh, smem, part);
+    constexpr FewSets sets = HP == 2 ? kTwoHeads : two ? kTwoBlocks : kOneSet;
+    few_item<T, D, (two ? 2 : ROWS / 16), sets, true>(p, 0, 0, 0, kvh, smem, part);
   }
   template <typename T, int D>
   static __device__ __forceinline__ void prefix(const SharedParams& p, int kvh, int piece, int tile, char* smem) {
@@ -74,6 +92,7 @@ struct Few {
 };
 template <int TP>
 struct Tile {
+  static constexpr int kRows = kPrefillRows;
   template <int D>
   static constexpr int bytes() { return 2 * PromptSmem<D, D, (TP > 1)>::kBytes; }
   template <typename T, int D>
@@ -197,6 +216,10 @@ static SharedPlan shared_plan(int32_t rows, int32_t queries, int32_t hq, int32_t
   SharedPlan s{};
   const int group = hq / hkv;
   const int64_t tokens = (int64_t)rows * queries, query_rows = tokens * group;
+  // Prompt items hold 128 rows; below, few-query items, which read no more than they need. 33 to 64 rows, few / prompt
+  // items, prefixes of 2K, 16K, 64K: d128 17.9 / 15.0, 31.2 / 25.9, 74.5 / 67.8 us; d64 12.8 / -, 18.7 / 17.8, 36.5 /
+  // 35.9. 17 to 32 rows at d128 13.0 / 13.9, 23.4 / 23.3, 55.3 / 63.2. On pages that 64-key tiles do not fit, few-query
+  // items of 64 rows whatever their number.
   if (query_rows > (d == 64 ? 64 : 32))
     s.tile_pages = block_size % 64 == 0 ? 1 : block_size == 32 ? 2 : block_size == 16 ? 4 : 0;
   s.tile_rows = s.tile_pages > 0 ? kPrefillRows / group * group : few_rows(query_rows);
@@ -207,6 +230,11 @@ static SharedPlan shared_plan(int32_t rows, int32_t queries, int32_t hq, int32_t
   const double own_us = (double)own_keys * hkv * d * 4 / kOwnBytesPerUs;
   s.per_piece = kPrefillKeys;
   if (shared > 0) {
+    // Pieces: one workgroup of the prefix per CU beside the own keys (few-query items always: their prefix streams too, 64K
+    // keys for 2 rows 50.6 us against 52.5 with two), or two where the own keys are worth less than what half the
+    // workgroups lose (256 rows on 64K tokens 349 -> 288). And no more than make a piece end within the own keys' time:
+    // each costs its partials' way through memory (128 rows on 2K tokens, 1 / 2 / 4 / 8 pieces 78 / 65 / 68 / 74 us; 64
+    // rows on 8K, 8 / 16 / 32 44 / 47 / 59).
     const int64_t units = (int64_t)s.tiles * hkv, key_tiles = (shared + kPrefillKeys - 1) / kPrefillKeys;
     const bool beside = s.tile_pages == 0 || own_us > 0.3 * (double)(units * key_tiles) / kTilesPerUs;
     int64_t want = (beside ? kSharedRound / 2 : kSharedRound) / units;
@@ -216,7 +244,10 @@ static SharedPlan shared_plan(int32_t rows, int32_t queries, int32_t hq, int32_t
     s.per_piece = (int32_t)(((shared + want - 1) / want + 63) / 64 * 64);
     s.pieces = (shared + s.per_piece - 1) / s.per_piece;
   }
-  s.own_heads = hkv % 2 == 0 && (int64_t)rows * hkv >= kSharedRound / 2 && queries * group <= 32 ? 2 : 1;
+  // Own keys: kv heads in pairs (512 adjacent bytes of a token) where those still make a workgroup for every second CU: 32
+  // rows on 8K tokens 39.3 -> 33.1 us, 4 rows of 8 kv heads 9.6 -> 11.4. Split to one round of a CU's second workgroups,
+  // or in two where there is more than a round (128 rows: one split 63.5, two 59.4, four 59.6), finer where rows are long.
+  s.own_heads = hkv % 2 == 0 && (int64_t)rows * hkv >= kSharedRound / 2 && queries * group <= 16 ? 2 : 1;
   const int64_t units = (int64_t)rows * hkv / s.own_heads, half = kSharedRound / 2;
   int64_t splits = units <= half ? half / units : 2;
   splits = std::max(splits, std::min<int64_t>((4 * kSharedRound + units - 1) / units, row_keys / 1024));
@@ -232,11 +263,12 @@ static SharedPlan shared_plan(int32_t rows, int32_t queries, int32_t hq, int32_t
 template <typename T, int D, typename PREFIX>
 static void launch_items(const SharedParams& p, int own_heads, hipStream_t stream) {
   const int rows = p.queries * p.group, prefix = p.pieces * p.tiles * p.hkv;
-  auto* const kernel = rows <= 16   ? (own_heads == 2 ? &shared_items_kernel<T, D, PREFIX, 16, 2>
-                                                      : &shared_items_kernel<T, D, PREFIX, 16, 1>)
-                       : rows <= 32 ? (own_heads == 2 ? &shared_items_kernel<T, D, PREFIX, 32, 2>
-                                                      : &shared_items_kernel<T, D, PREFIX, 32, 1>)
-                                    : &shared_items_kernel<T, D, PREFIX, 64, 1>;
+  auto* kernel = own_heads == 2 ? &shared_items_kernel<T, D, PREFIX, 16, 2> : &shared_items_kernel<T, D, PREFIX, 16, 1>;
+  // A prefix of few-query items has at least as many rows as one of its rows' own.
+  if constexpr (PREFIX::kRows >= 32)
+    if (rows > 16) kernel = &shared_items_kernel<T, D, PREFIX, 32, 1>;
+  if constexpr (PREFIX::kRows >= 64)
+    if (rows > 32) kernel = &shared_items_kernel<T, D, PREFIX, 64, 1>;
   hipLaunchKernelGGL(kernel, dim3(prefix + p.splits * p.rows * (p.hkv / own_heads)), dim3(256), 0, stream, p, prefix);
 }
 

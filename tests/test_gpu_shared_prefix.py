@@ -121,6 +121,27 @@ def test_matches_attention_row_by_row(cuda, shared, owns, queries, hq, hk, dim, 
     close(attend(cuda, shared, *s, scale), *want(*s, queries, scale))
 
 
+# The kernels of a call: how the prefix is computed (few-query items of 16, 32 or 64 rows, or prompt items on pages of
+# 64, 32 or 16), and the rows' own keys (16, 32 or 64 rows, or 16 of a pair of kv heads). rows, queries, hq, hk, page.
+KERNELS = {
+    "few16-16": (4, 1, 8, 4, 64), "few16-pairs": (8, 1, 32, 32, 16), "few32-16": (10, 1, 8, 4, 32),
+    "few32-32": (1, 3, 16, 2, 16), "few32-pairs": (16, 1, 32, 16, 64), "few64-16": (40, 1, 2, 1, 48),
+    "few64-pairs": (40, 1, 16, 8, 48), "few64-32": (5, 3, 8, 1, 48), "few64-64": (5, 5, 16, 2, 48),
+    **{f"tile{page}-{own}": (*shape, page) for page in (64, 32, 16) for own, shape in
+       {"16": (40, 1, 2, 1), "pairs": (40, 1, 16, 8), "32": (5, 3, 8, 1), "64": (5, 5, 16, 2)}.items()}}
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("name", KERNELS)
+def test_every_kernel(cuda, name, dtype, dim):
+    rows, queries, hq, hk, page = KERNELS[name]
+    owns = [queries + (37 * i) % 70 for i in range(rows)]
+    owns[-1] = 530  # two splits of a row's own keys
+    s = step(576, owns, hq=hq, hk=hk, dim=dim, page=page, dtype=dtype, queries=queries, seed=rows)
+    close(attend(cuda, 576, *s, dim ** -0.5), *want(*s, queries, dim ** -0.5))
+
+
 @pytest.mark.parametrize("dim,page,rows", [(128, 16, 5), (64, 256, 5), (128, 48, 5), (128, 64, 70)])
 def test_rows_that_do_not_see_the_prefix(cuda, dim, page, rows):
     """Padding rows get zeros; a row shorter than the shared keys is attended by itself through its own table, whatever
