@@ -26,15 +26,19 @@ LV_PACK_DENSE_SLOTS = 1
 
 class DecodeGraphs:
     """Captured decode steps of ``query_len`` queries per row, one graph per batch size (smallest that fits is
-    replayed). ``max_blocks`` bounds every row's block list (``model_runner.py:661-667``)."""
+    replayed). ``max_blocks`` bounds every row's block list (``model_runner.py:661-667``). ``rotary``: None where the
+    queries and keys come rotated; else what ``append_kvcache`` takes beside them (``table``, and ``q_weight``,
+    ``k_weight``, ``eps``, ``interleaved``), which then takes the store's place in the graph: at the positions that the
+    pack kernel writes there."""
 
     def __init__(self, backend: MI355XAttention, k_cache: torch.Tensor, v_cache: torch.Tensor, batch_sizes,
-                 max_blocks: int, query_len: int = 1):
+                 max_blocks: int, query_len: int = 1, rotary: dict | None = None):
         self.backend, self.k_cache, self.v_cache = backend, k_cache, v_cache
         self.device = k_cache.device
         self.block_size = k_cache.size(1)
         self.sizes = sorted(set(int(b) for b in batch_sizes))
         self.max_blocks, self.query_len = int(max_blocks), int(query_len)
+        self.rotary = rotary
         max_bs = self.sizes[-1]
         tokens = max_bs * self.query_len
         heads, kv_heads, dim = backend.num_heads, backend.num_kv_heads, backend.head_dim
@@ -90,16 +94,21 @@ class DecodeGraphs:
                    self.cu_seqlens_k.data_ptr(), self.positions.data_ptr(), self.slot_mapping.data_ptr(),
                    self.context_lens.data_ptr(), self.block_tables.data_ptr(), None, None, None, LV_PACK_DENSE_SLOTS,
                    _capi.stream_of(self.device))
-        self.backend.store_kvcache(self.k[:tokens], self.v[:tokens], self.k_cache, self.v_cache,
-                                   self.slot_mapping[:tokens])
+        q_step = self.q[:tokens]
+        if self.rotary is None:
+            self.backend.store_kvcache(self.k[:tokens], self.v[:tokens], self.k_cache, self.v_cache,
+                                       self.slot_mapping[:tokens])
+        else:
+            q_step = self.backend.append_kvcache(q_step, self.k[:tokens], self.v[:tokens], self.k_cache, self.v_cache,
+                                                 self.slot_mapping[:tokens], self.positions[:tokens], **self.rotary)
         ctx = Context(is_prefill=q > 1, cu_seqlens_q=self.cu_seqlens_q[:bs + 1],
                       cu_seqlens_k=self.cu_seqlens_k[:bs + 1], max_seqlen_q=q, max_seqlen_k=w * self.block_size,
                       slot_mapping=self.slot_mapping[:tokens], context_lens=self.context_lens[:bs],
                       block_tables=self.block_tables[:bs * w].view(bs, w))
         if q == 1:
-            self.backend.decode(self.q[:tokens], self.k_cache, self.v_cache, ctx, out=self.out[:tokens])
+            self.backend.decode(q_step, self.k_cache, self.v_cache, ctx, out=self.out[:tokens])
         else:
-            self.backend.prefill(self.q[:tokens], None, None, self.k_cache, self.v_cache, ctx, out=self.out[:tokens])
+            self.backend.prefill(q_step, None, None, self.k_cache, self.v_cache, ctx, out=self.out[:tokens])
 
     def capture(self) -> None:
         """Capture every batch size, largest first, each after an eager warmup on padding rows (which grows the

@@ -221,3 +221,39 @@ def test_append_replays_in_a_graph_and_on_another_stream(cuda):
             again = backend.append_kvcache(q, k, v, *eager, slots, pos, table)
         side.synchronize()
         assert torch.equal(out, again) and all(torch.equal(a, b) for a, b in zip(caches, eager))
+
+
+@pytest.mark.parametrize("query_len", [1, 3], ids=["decode", "drafts"])
+def test_decode_graphs_rotate_inside(cuda, query_len):
+    """DecodeGraphs with a rotary table: a replay of raw projections equals rotating them into the cache and attending
+    eagerly, bit for bit in the cache and the queries' attention, with padding rows that store nothing."""
+    hq, hk, dim, bs, blocks, most = 8, 2, 128, 16, 48, 6
+    backend, dt = lvattn.MI355XAttention(hq, dim, 0.09, hk), torch.bfloat16
+    gen = torch.Generator().manual_seed(query_len)
+    caches = [torch.randn(blocks, bs, hk, dim, generator=gen).to(dt).to(cuda) for _ in range(2)]
+    w = (1 + 0.2 * torch.randn(dim, generator=gen)).to(dt).to(cuda)
+    rotary = dict(table=lvattn.rotary_table(dim, 256, device=cuda), q_weight=w, k_weight=w, eps=1e-5)
+    graphs = lvattn.DecodeGraphs(backend, *caches, [4, 8], most, query_len, rotary=rotary)
+    before = [c.clone() for c in caches]
+    graphs.capture()
+    assert all(torch.equal(a, b) for a, b in zip(caches, before))  # padding rows only
+    packer = lvattn.Packer(cuda, bs)
+    for turn, rows in enumerate((3, 8, 1, 4)):
+        pages = torch.randperm(blocks, generator=gen)[:rows * most].view(rows, most).tolist()
+        cached = torch.randint(0, most * bs - query_len + 1, (rows,), generator=gen).tolist()
+        lists = [p[:-(-(c + query_len) // bs)] for p, c in zip(pages, cached)]
+        t = rows * query_len
+        q, k, v = (torch.randn(t, h, dim, generator=gen).to(dt).to(cuda) for h in (hq, hk, hk))
+        eager = [c.clone() for c in caches]
+        got = graphs.replay(cached, lists, q, k, v).clone()
+        positions, fields = packer.pack(cached, [query_len] * rows, lists, num_speculative_tokens=query_len - 1,
+                                        is_prompt=[False] * rows)
+        fields.pop("order")
+        ctx = lvattn.Context(**fields)
+        turned = backend.append_kvcache(q, k, v, *eager, ctx.slot_mapping, positions, **rotary)
+        assert all(torch.equal(a, b) for a, b in zip(caches, eager))
+        y, size = R.rotate(q.cpu(), positions.cpu(), dim, weight=w.cpu(), eps=1e-5)
+        close(turned, y, size)
+        want = backend.forward(turned, k, v, *eager, ctx)
+        # the graph's bound on the keys may split them otherwise: the outputs' own tolerance in this repository
+        torch.testing.assert_close(got.float(), want.float(), atol=2e-2, rtol=1e-2)
