@@ -331,7 +331,9 @@ class MI355XAttention(AttentionBackend):
         keys is attended by itself; one of no keys (graph padding) gets zeros. Nothing is read back, so a call can be
         captured (a graph keeps ``shared_len``)."""
         what = "decode_shared"
-        bt, lens = context.block_tables, context.context_lens
+        bt, lens, shared_len = context.block_tables, context.context_lens, int(shared_len)
+        if bt is None or lens is None or bt.dim() != 2:
+            raise ValueError(f"{what}: the context has no block tables [rows, pages] or no context lengths")
         tokens, heads, dim = q.shape
         kv_heads, dtype, device, qs = self.num_kv_heads, q.dtype, q.get_device(), q.stride()
         shape, cs = k_cache.shape, k_cache.stride()
@@ -354,7 +356,8 @@ class MI355XAttention(AttentionBackend):
                              "pages")
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif out.shape != q.shape or out.dtype is not dtype or out.stride(2) != 1 or out.get_device() != device:
+        elif (out.shape != q.shape or out.dtype is not dtype or out.stride(2) != 1 or out.get_device() != device
+              or (out.stride(0) == 0 and tokens > 1) or (out.stride(1) == 0 and heads > 1)):
             raise ValueError(f"{what}: out is {out.dtype} {tuple(out.shape)}, not {dtype} {tuple(q.shape)} beside q")
         if device < 0 or not (k_cache.get_device() == v_cache.get_device() == bt.get_device() == lens.get_device()
                               == device):

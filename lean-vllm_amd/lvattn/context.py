@@ -94,7 +94,7 @@ def shared_prefix_len(block_lists, num_cached, block_size: int) -> int:
         raise ValueError(f"shared_prefix_len: {len(block_lists)} block lists for {len(num_cached)} rows")
     if len(block_lists) < 2:
         return 0
-    most = min(min(num_cached) // block_size, min(len(b) for b in block_lists))
+    most = min(int(min(num_cached)) // block_size, min(len(b) for b in block_lists))
     first = block_lists[0]
     # The shared pages lead: found by bisection, a slice compared per row and step.
     lo, hi = 0, most

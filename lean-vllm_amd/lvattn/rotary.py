@@ -26,7 +26,10 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
     - ``llama3``: pairs of fewer than ``low_freq_factor`` (1) turns over ``original_max_position_embeddings`` slowed by
       ``factor``, of more than ``high_freq_factor`` (4) kept, a linear blend between;
     - ``yarn`` (Peng et al., "YaRN", 2023): the blend linear over the pairs' indices, from ``beta_fast`` (32) turns to
-      ``beta_slow`` (1), and cosines and sines times ``attention_factor`` (``0.1 ln(factor) + 1``).
+      ``beta_slow`` (1), at whole indices unless ``truncate`` is False, and cosines and sines times ``attention_factor``:
+      by default ``a(1)`` with ``a(m) = 0.1 m ln(factor) + 1``, or ``a(mscale) / a(mscale_all_dim)`` where both are given.
+
+    Other keys are refused: one that is ignored would give other angles than the checkpoint's.
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_frequencies: the rotary width {rotary_dim} is not a positive even number")
@@ -34,12 +37,19 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
         raise ValueError(f"rotary_frequencies: base {base} is not above 1")
     r, s = rotary_dim, dict(scaling or {})
     kind = s.pop("rope_type", None) or s.pop("type", None) or "default"
+    keys = {"default": (), "linear": ("factor",), "ntk": ("factor",),
+            "llama3": ("factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor"),
+            "yarn": ("factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "truncate",
+                     "attention_factor", "mscale", "mscale_all_dim")}
+    if kind not in keys:
+        raise ValueError(f"rotary_frequencies: rope_type {kind!r} is not one of {', '.join(keys)}")
+    other = sorted(set(s) - set(keys[kind]))
+    if other:
+        raise ValueError(f"rotary_frequencies: rope_type {kind!r} takes no {', '.join(other)}")
     exponents = np.arange(0, r, 2, dtype=np.float64) / r
     inv = float(base) ** -exponents
     if kind == "default":
         return inv, 1.0
-    if kind not in ("linear", "ntk", "llama3", "yarn"):
-        raise ValueError(f"rotary_frequencies: rope_type {kind!r} is not one of default, linear, ntk, llama3, yarn")
     factor = float(s.get("factor", 0.0))
     if not factor >= 1.0:
         raise ValueError(f"rotary_frequencies: rope_type {kind!r} needs a factor of at least 1, got {s.get('factor')}")
@@ -65,10 +75,20 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
     fast, slow = float(s.get("beta_fast") or 32.0), float(s.get("beta_slow") or 1.0)
     if not 0 < slow < fast:
         raise ValueError(f"rotary_frequencies: beta_fast {fast} and beta_slow {slow}")
-    lo, hi = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), r - 1)
+    lo, hi = pair_of(fast), pair_of(slow)
+    if s.get("truncate", True):
+        lo, hi = math.floor(lo), math.ceil(hi)
+    lo, hi = max(lo, 0), min(hi, r - 1)
     slowed = np.clip((np.arange(r // 2) - lo) / max(hi - lo, 1e-3), 0.0, 1.0)
+
+    def a(m: float) -> float:
+        return 0.1 * m * math.log(factor) + 1.0
+
     amp = s.get("attention_factor")
-    return inv * (1.0 - slowed + slowed / factor), float(amp) if amp is not None else 0.1 * math.log(factor) + 1.0
+    if amp is None:
+        both = s.get("mscale") and s.get("mscale_all_dim")
+        amp = a(float(s["mscale"])) / a(float(s["mscale_all_dim"])) if both else a(1.0)
+    return inv * (1.0 - slowed + slowed / factor), float(amp)
 
 
 def rotary_table(rotary_dim: int, max_position: int, base: float = 10000.0, scaling: dict | None = None,
@@ -144,6 +164,8 @@ def output_heads(what: str, name: str, x, out, like: tuple):
     if x is None or out.shape != x.shape:
         raise ValueError(f"{what}: {name} is {tuple(out.shape)}, its input "
                          f"{'missing' if x is None else tuple(x.shape)}")
+    if (out.stride(0) == 0 and out.size(0) > 1) or (out.stride(1) == 0 and out.size(1) > 1):
+        raise ValueError(f"{what}: {name} of strides {out.stride()} holds one row for several heads or tokens")
     return out, head_args(what, name, out, *like)[:3]
 
 

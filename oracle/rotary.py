@@ -30,12 +30,20 @@ def angles(rotary_dim: int, base: float, scaling: dict | None = None) -> tuple[l
             def edge(turns):  # where base ** (-2 x / r) makes `turns` turns over the trained length, in halves of x
                 return rotary_dim / 2 * math.log(trained / (turns * 2 * math.pi), base)
 
-            lo = max(math.floor(edge(s.get("beta_fast", 32))), 0)
-            hi = min(math.ceil(edge(s.get("beta_slow", 1))), rotary_dim - 1)
+            down, up = (math.floor, math.ceil) if s.get("truncate", True) else (float, float)
+            lo = max(down(edge(s.get("beta_fast", 32))), 0)
+            hi = min(up(edge(s.get("beta_slow", 1))), rotary_dim - 1)
             share = 0.0 if i <= lo else 1.0 if i >= hi else (i - lo) / (hi - lo)
             w = w / factor * share + w * (1 - share)
         out.append(w)
-    return out, (s.get("attention_factor") or 0.1 * math.log(factor) + 1) if kind == "yarn" else 1.0
+    if kind != "yarn":
+        return out, 1.0
+    if "attention_factor" in s:
+        return out, s["attention_factor"]
+    ln = math.log(factor)
+    if "mscale" in s and "mscale_all_dim" in s:
+        return out, (0.1 * s["mscale"] * ln + 1) / (0.1 * s["mscale_all_dim"] * ln + 1)
+    return out, 0.1 * ln + 1
 
 
 def rotate(x, positions, rotary_dim: int, base: float = 10000.0, scaling: dict | None = None, interleaved: bool = False,

@@ -116,6 +116,19 @@ def test_odd_positions(cuda):
         assert y[[1, 3], :, :rot].isnan().all() and y[2].isfinite().all()
 
 
+def test_views_of_part_of_a_head_in_place(cuda):
+    """Latent attention's rope dims: the last 64 of 192-wide query heads and of 576-wide latents, in place, interleaved; the
+    other dims stay."""
+    q, latent = (torch.randn(9, *shape, device=cuda).to(torch.bfloat16) for shape in ((16, 192), (576,)))
+    table, pos = lvattn.rotary_table(64, 500, device=cuda), torch.arange(9, device=cuda) * 50
+    want_q, want_l = q.clone(), latent.clone()
+    rope = [q[..., 128:], latent[:, None, 512:]]
+    lvattn.apply_rotary(*rope, pos, table, interleaved=True, out_q=rope[0], out_k=rope[1])
+    for got, x, n in ((q, want_q, 128), (latent[:, None], want_l[:, None], 512)):
+        assert torch.equal(got[..., :n], x[..., :n])
+        close(got[..., n:], *R.rotate(x[..., n:].cpu(), pos.cpu(), 64, interleaved=True))
+
+
 def test_not_a_number_stays_in_its_head(cuda):
     q = torch.randn(6, 8, 128, device=cuda).to(torch.bfloat16)
     w, table = torch.ones(128, device=cuda, dtype=torch.bfloat16), lvattn.rotary_table(128, 10, device=cuda)

@@ -14,7 +14,9 @@ SCALINGS = [None, dict(rope_type="linear", factor=4.0), dict(rope_type="ntk", fa
                  original_max_position_embeddings=8192),
             dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=32768),
             dict(rope_type="yarn", factor=40.0, original_max_position_embeddings=4096, beta_fast=32, beta_slow=1,
-                 attention_factor=1.0)]
+                 attention_factor=1.0),
+            dict(rope_type="yarn", factor=40.0, original_max_position_embeddings=4096, mscale=1.0, mscale_all_dim=0.707),
+            dict(rope_type="yarn", factor=16.0, original_max_position_embeddings=4096, truncate=False)]
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
@@ -71,6 +73,7 @@ def test_the_ends_of_the_scalings():
 @pytest.mark.parametrize("args,message", [
     ((7,), "not a positive even"), ((0,), "not a positive even"), ((8, 1.0), "not above 1"),
     ((8, 1e4, dict(rope_type="spline", factor=2.0)), "rope_type 'spline'"),
+    ((8, 1e4, dict(rope_type="linear", factor=2.0, mscale=1.0)), "takes no mscale"), ((8, 1e4, dict(factor=2.0)), "takes no"),
     ((8, 1e4, dict(rope_type="linear")), "factor of at least 1"),
     ((8, 1e4, dict(rope_type="linear", factor=0.5)), "factor of at least 1"),
     ((2, 1e4, dict(rope_type="ntk", factor=2.0)), "width above 2"),
@@ -113,6 +116,16 @@ POS, TABLE = torch.zeros(4, dtype=torch.int64), torch.zeros(32, 16)
 def test_calls_refuse(q, k, positions, table, message):
     with pytest.raises(ValueError, match=message):
         lvattn.apply_rotary(q, k, positions, table)
+
+
+def test_outputs_refuse():
+    for out, message in ((heads(t=3), "out_q is"), (heads(dtype=torch.float16), "must be on one GPU|out_q is"),
+                         (heads(t=1).expand(4, 2, 16), "holds one row")):
+        q = heads()
+        with pytest.raises(ValueError, match=message):
+            lvattn.rotary.output_heads("apply_rotary", "out_q", q, out, (4, 16, torch.bfloat16, -1))
+    with pytest.raises(ValueError, match="its input missing"):
+        lvattn.rotary.output_heads("apply_rotary", "out_k", None, heads(), (4, 16, torch.bfloat16, -1))
 
 
 def test_norms_and_appends_refuse():

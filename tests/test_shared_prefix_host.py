@@ -19,7 +19,8 @@ def test_shared_prefix_len():
     assert shared_prefix_len([head, head[:3] + [2]], [64, 64], 16) == 48
     assert shared_prefix_len([head, []], [64, 0], 16) == 0
     assert shared_prefix_len([head], [64], 16) == 0 and shared_prefix_len([], [], 16) == 0
-    assert shared_prefix_len([np.array(head), tuple(head)], np.array([64, 64]), 16) == 64
+    got = shared_prefix_len([np.array(head), tuple(head)], np.array([64, 64]), 16)
+    assert got == 64 and type(got) is int
     for n in range(12):  # against the definition, over lengths
         a, b = list(range(12)), list(range(n)) + [99] * (12 - n)
         assert shared_prefix_len([a, b, a], [12 * 8] * 3, 8) == 8 * n
@@ -54,8 +55,13 @@ def test_the_call_refuses_lengths_and_outputs():
     for bad in (-16, 8, 112):
         with pytest.raises(ValueError, match=f"{bad} shared keys"):
             backend.decode_shared(**(a | dict(shared_len=bad)))
-    with pytest.raises(ValueError, match="out is"):
-        backend.decode_shared(**a, out=torch.zeros(4, 8, 128, dtype=BF))
+    for out in (torch.zeros(4, 8, 128, dtype=BF), torch.zeros(1, 8, 64, dtype=BF).expand(4, 8, 64)):
+        with pytest.raises(ValueError, match="out is"):
+            backend.decode_shared(**a, out=out)
+    for context in (Context(), Context(block_tables=a["context"].block_tables),
+                    Context(block_tables=torch.zeros(4, dtype=torch.int32), context_lens=a["context"].context_lens)):
+        with pytest.raises(ValueError, match="no block tables"):
+            backend.decode_shared(**(a | dict(context=context)))
 
 
 def test_the_debug_check_finds_pages_that_are_not_shared():
