@@ -16,8 +16,8 @@
 // (prefix keys, rows, own keys a row; us):
 //                                         one launch      prefix, own and merge launches   lv_paged_attention
 //   32,768, 200 rows, 64-2048             231             303                              2380
-//   8192, 64 rows, 16-1024                46.8            60.8                             244
-//   2048, 128 rows, 64-1024, 16 a page    64.6            80.4                             149
+//   8192, 64 rows, 16-1024                43.1            60.8                             244
+//   2048, 128 rows, 64-1024, 16 a page    63.8            80.4                             149
 //   65,536, 256 rows, 16-64               287             312                              5786
 //   16,384, 16 rows, 64-512               24.9            38.6                             123
 // What is left at 200 rows: the prefix alone takes 134 us on whole CUs and 179 on one workgroup of each, the own keys alone
@@ -28,18 +28,19 @@
 namespace lv {
 
 constexpr int kSharedRound = 512;      // workgroups that run at once (two per CU)
-constexpr int kOwnKeys = 256;          // least keys a row's own split is cut for
 constexpr int kSharedPieceKeys = 256;  // and a piece of the prefix
 constexpr int kMaxOwnSplits = 32;
 constexpr int kMaxSharedPieces = 256;
-// 64-key tiles of prompt items that the GPU takes in a microsecond with two workgroups on each CU (245; 190 with one), and
-// one such workgroup's time for a tile; the rate at which own keys stream. 32/8 heads of 128 and 64/8 of 64.
-constexpr double kTilesPerUs = 245, kTileUs = 1.32, kOwnBytesPerUs = 6.0e6;
+// 64-key tiles of prompt items that the GPU takes in a microsecond with two workgroups on each CU (245; 190 with one); a
+// workgroup's time for a tile beside own items (1.3 alone on its CU); the rate at which own keys stream, and what their
+// items take besides. 32/8 heads of 128 and 64/8 of 64.
+constexpr double kTilesPerUs = 245, kTileUs = 2.0, kOwnBytesPerUs = 6.0e6, kOwnStartUs = 10;
 
 struct SharedParams : AttnParams {
   int32_t shared, queries, tokens;  // keys of the prefix; queries per row; all queries
   int32_t tile_rows, tiles;         // (query, head) rows of a prefix tile, tiles per kv head
-  int32_t per_piece, splits;        // keys per piece (p.pieces of them); most splits of a row's own keys
+  int32_t per_piece;                // keys per piece (p.pieces of them)
+  int32_t splits, own_least;        // most splits of a row's own keys, and the least keys that one is cut for
 };
 
 // A row's own part: its keys from `start` on, in `n` splits of `per` (none where the row has no keys). A row that does not
@@ -51,7 +52,7 @@ __device__ __forceinline__ OwnSpan own_span(const SharedParams& p, int len) {
   OwnSpan s;
   s.start = len - p.queries + 1 >= p.shared ? p.shared : 0;
   const int keys = len - s.start;
-  const int want = min(p.splits, (keys + kOwnKeys - 1) / kOwnKeys);
+  const int want = min(p.splits, (keys + p.own_least - 1) / p.own_least);
   s.per = want > 1 ? ((keys + want - 1) / want + 63) / 64 * 64 : max(keys, 1);
   s.n = keys > 0 ? (keys + s.per - 1) / s.per : 0;
   return s;
@@ -204,7 +205,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedParams p) {
 // What the host decides from the shapes.
 struct SharedPlan {
   int32_t tile_pages;  // pages per 64-key tile of prompt items (0: few-query items)
-  int32_t tile_rows, tiles, pieces, per_piece, splits, own_heads;
+  int32_t tile_rows, tiles, pieces, per_piece, splits, own_least, own_heads;
   size_t o_bytes, bytes;  // partial outputs, then their log-sum-exps
 };
 
@@ -233,27 +234,31 @@ static SharedPlan shared_plan(int32_t rows, int32_t queries, int32_t hq, int32_t
     // Pieces: one workgroup of the prefix per CU beside the own keys (few-query items always: their prefix streams too, 64K
     // keys for 2 rows 50.6 us against 52.5 with two), or two where the own keys are worth less than what half the
     // workgroups lose (256 rows on 64K tokens 349 -> 288). And no more than make a piece end within the own keys' time:
-    // each costs its partials' way through memory (128 rows on 2K tokens, 1 / 2 / 4 / 8 pieces 78 / 65 / 68 / 74 us; 64
-    // rows on 8K, 8 / 16 / 32 44 / 47 / 59).
+    // each costs its partials' way through memory (128 rows on 2K tokens, 1 / 2 / 4 / 8 pieces 78 / 65 / 68 / 74 us; 256
+    // on 1K, 1 / 2 / 4 / 8 68 / 74 / 78 / 85; 64 rows on 8K, 8 / 16 / 32 43 / 47 / 59).
     const int64_t units = (int64_t)s.tiles * hkv, key_tiles = (shared + kPrefillKeys - 1) / kPrefillKeys;
     const bool beside = s.tile_pages == 0 || own_us > 0.3 * (double)(units * key_tiles) / kTilesPerUs;
     int64_t want = (beside ? kSharedRound / 2 : kSharedRound) / units;
     if (s.tile_pages > 0 && beside)
-      want = std::min(want, (int64_t)std::ceil((double)key_tiles * kTileUs / std::max(0.75 * own_us, 8.0)));
+      want = std::min(want, (int64_t)std::ceil((double)key_tiles * kTileUs / (own_us + kOwnStartUs)));
     want = std::max<int64_t>(1, std::min<int64_t>({want, kMaxSharedPieces, shared / kSharedPieceKeys}));
     s.per_piece = (int32_t)(((shared + want - 1) / want + 63) / 64 * 64);
     s.pieces = (shared + s.per_piece - 1) / s.per_piece;
   }
   // Own keys: kv heads in pairs (512 adjacent bytes of a token) where those still make a workgroup for every second CU: 32
-  // rows on 8K tokens 39.3 -> 33.1 us, 4 rows of 8 kv heads 9.6 -> 11.4. Split to one round of a CU's second workgroups,
-  // or in two where there is more than a round (128 rows: one split 63.5, two 59.4, four 59.6), finer where rows are long.
+  // rows on 8K tokens 39.3 -> 33.1 us, 4 rows of 8 kv heads 9.6 -> 11.4. Split to one round of the workgroups that the
+  // prefix leaves (64 rows on 8K: one split 49, two 43), or in two where there is more than a round (128 rows alone: one
+  // split 63.5, two 59.4, four 59.6), finer where rows are long. A split holds at least 384 keys where workgroups are
+  // many (256 rows on 1K 68.5 -> 67), 256 where they are few (4 rows 10.5 -> 9.7).
   s.own_heads = hkv % 2 == 0 && (int64_t)rows * hkv >= kSharedRound / 2 && queries * group <= 16 ? 2 : 1;
-  const int64_t units = (int64_t)rows * hkv / s.own_heads, half = kSharedRound / 2;
-  int64_t splits = units <= half ? half / units : 2;
+  const int64_t units = (int64_t)rows * hkv / s.own_heads;
+  const int64_t beside = std::max<int64_t>(kSharedRound - (int64_t)s.pieces * s.tiles * hkv, kSharedRound / 2);
+  int64_t splits = units < beside ? (beside + units / 2) / units : 2;
   splits = std::max(splits, std::min<int64_t>((4 * kSharedRound + units - 1) / units, row_keys / 1024));
+  s.own_least = 2 * units <= beside ? 256 : 384;
   // A row that does not see the prefix walks all its keys, so the bound is on those, not on the keys behind it.
   s.splits = (int32_t)std::max<int64_t>(
-      1, std::min<int64_t>({splits, kMaxOwnSplits, ((int64_t)max_k + kOwnKeys - 1) / kOwnKeys}));
+      1, std::min<int64_t>({splits, kMaxOwnSplits, ((int64_t)max_k + s.own_least - 1) / s.own_least}));
   const int64_t partials = ((int64_t)s.pieces + s.splits) * tokens * hq;
   s.o_bytes = (size_t)partials * d * sizeof(float);
   s.bytes = s.o_bytes + (size_t)partials * sizeof(float);
@@ -386,6 +391,7 @@ extern "C" int lv_shared_prefix_decode(const void* q, int64_t q_stride_t, int64_
   p.tiles = s.tiles;
   p.per_piece = s.per_piece;
   p.splits = s.splits;
+  p.own_least = s.own_least;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (dtype == LV_DTYPE_BF16)
     return head_dim == 64 ? launch_shared<BF16, 64>(p, s, st) : launch_shared<BF16, 128>(p, s, st);
