@@ -105,8 +105,8 @@ int lv_store_latents(const void* latent, int64_t latent_stride_t, int32_t num_to
  * q_weight / k_weight (either may be NULL: not normed): [D] of the same dtype, contiguous; x is first
  *   x * rsqrt(mean(x^2) + eps) * weight.
  * Computed in fp32, rounded once. q_out, k_out: same shapes, own strides; each may be its input (the same pointer and
- * strides), and must not overlap it otherwise. A negative position (a captured step's padding row) rotates as position 0; one at or
- * past max_position gives NaN in the rotated dims. */
+ * strides), and must not overlap it otherwise. A negative position (a captured step's padding row) rotates as position
+ * 0; one at or past max_position gives NaN in the rotated dims. */
 int lv_rotary(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
               int64_t k_stride_h, const int64_t* positions, const float* table, int64_t max_position,
               int32_t rotary_dim, int32_t interleaved, const void* q_weight, const void* k_weight, float eps,
@@ -267,8 +267,8 @@ int lv_shared_prefix_decode(const void* q, int64_t q_stride_t, int64_t q_stride_
                             int64_t table_stride, const int32_t* context_lens, int32_t num_rows,
                             int32_t queries_per_row, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                             float scale, int32_t shared_len, int32_t max_seqlen_k, int64_t own_keys, void* out,
-                            int64_t out_stride_t, int64_t out_stride_h, void* workspace, size_t workspace_bytes, int32_t dtype,
-                            void* stream);
+                            int64_t out_stride_t, int64_t out_stride_h, void* workspace, size_t workspace_bytes,
+                            int32_t dtype, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------
  * Attention over packed keys (no pages). Replaces AttentionBackend.prefill without block tables and

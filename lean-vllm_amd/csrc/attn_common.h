@@ -192,7 +192,8 @@ __device__ void prefill_item(const AttnParams& p, int row, int qtile, int kvh, c
   static_assert(!SPLIT || (RING > 0 && !CTX && WAVES == 4), "split items stream paged keys");
   const int per_piece = SPLIT ? (all_tiles + p.pieces - 1) / p.pieces : all_tiles;
   const int tile0 = PART ? part.tile0 : SPLIT ? min(piece * per_piece, all_tiles) : 0;
-  const int ntiles = PART ? part.tile0 + part.tiles : SPLIT ? min(tile0 + per_piece, all_tiles) : all_tiles;  // this call's tiles: tile0 .. ntiles - 1
+  // This call's tiles: tile0 .. ntiles - 1.
+  const int ntiles = PART ? part.tile0 + part.tiles : SPLIT ? min(tile0 + per_piece, all_tiles) : all_tiles;
 
   float m[2], l[2];  // raw-score max (held or running) and row sums
   f32x4 o[2][DB];

@@ -1,5 +1,5 @@
-// The item of paged attention of rows with few queries on MFMA: drafted tokens (2 to 16 queries a row), and decode rows whose GQA
-// group is not 1, 2 or 4 query heads.
+// The item of paged attention of rows with few queries on MFMA: drafted tokens (2 to 16 queries a row), and decode
+// rows whose GQA group is not 1, 2 or 4 query heads.
 //
 // An item is (row, split, kv head): all of the row's (position, head) query rows of one GQA group, up to 64, against
 // the keys [split * S, (split + 1) * S) of the row, so the keys and values are read from memory once. Bound by HBM:
@@ -159,7 +159,8 @@ __device__ __forceinline__ void few_item(const AttnParams& p, int row, int split
 #pragma unroll
       for (int k = 0; k < KS; ++k) qb[nb][k] = in ? ld16(src + 64 * k) : u32x4{0, 0, 0, 0};
     }
-    const int all = PART && !part.causal ? lk : lk - lq + q0 / G + 1;  // keys below it are seen by every query row of the pass
+    // Keys below it are seen by every query row of the pass.
+    const int all = PART && !part.causal ? lk : lk - lq + q0 / G + 1;
     float m[NB], l[NB];
     f32x4 o[NB][DB];
 #pragma unroll

@@ -111,15 +111,17 @@ __global__ __launch_bounds__(256) void rotary_any_kernel(RotaryParams p, int32_t
   for (int d = p.rot + lane; d < p.dim; d += 64) store1<T>(r.dst, d, normed(d));
 }
 
-// Rows of whole 16-byte chunks: LPH lanes a head row, each two chunks that hold both elements of every pair in them (half
-// layout: chunks c and c + r / 16; interleaved, and behind the rotary width: c and the one as many further on as there
-// are such lanes, so that neighbouring lanes' chunks lie side by side: two adjacent chunks a lane took 43.3 us where
-// these take 37.3, 8192 tokens interleaved), so a row is read once, turned in registers and written once. A wave takes kRounds rounds of 64 / LPH head rows of one token,
-// their loads all issued before the first is used, and the table's 8 cosines and 8 sines a lane once for all rounds.
+// Rows of whole 16-byte chunks: LPH lanes a head row, each two chunks that hold both elements of every pair in them
+// (half layout: chunks c and c + r / 16; interleaved, and behind the rotary width: c and the one as many further on as
+// there are such lanes, so that neighbouring lanes' chunks lie side by side: two adjacent chunks a lane took 43.3 us
+// where these take 37.3, 8192 tokens interleaved), so a row is read once, turned in registers and written once. A wave
+// takes kRounds rounds of 64 / LPH head rows of one token, their loads all issued before the first is used, and the
+// table's 8 cosines and 8 sines a lane once for all rounds.
 //
 // Measured on 32/8 heads of 128, bf16, normed, into the cache: 8192 tokens 36.7 us, 5.60 TB/s (a 1 GiB copy: 5.25);
-// normed only, 16384 tokens 60.3 us, 5.71 TB/s; 1 to 100 tokens 4 us, a launch and three dependent loads (position, table
-// row, and under them the head rows). One, two, three and four rounds a wave: 8192 tokens 44.6 / 40.7 / 44.6 / 42.1 us.
+// normed only, 16384 tokens 60.3 us, 5.71 TB/s; 1 to 100 tokens 4 us, a launch and three dependent loads (position,
+// table row, and under them the head rows). One, two, three and four rounds a wave: 8192 tokens 44.6 / 40.7 / 44.6 /
+// 42.1 us.
 //
 // STREAM: loads and stores past the caches. A step's q, k and v come from the projection before and go to the attention
 // after, so a call that fits the 256 MB Infinity Cache leaves its outputs there; one that does not only evicts. A
@@ -237,9 +239,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int32_t hea
   }
 }
 
-// The same rows with a rotary width that is no multiple of 16 (interleaved: 8), so that a pair's elements lie in other lanes (quarters
-// of 80- and 96-wide heads: 20 and 24): a lane holds two adjacent chunks and takes its elements' partners from the LDS. 8192 tokens, 32/8 heads of 80 of which 20 turn, normed
-// 52 us, rotary_any_kernel 140.
+// The same rows with a rotary width that is no multiple of 16 (interleaved: 8), so that a pair's elements lie in other
+// lanes (quarters of 80- and 96-wide heads: 20 and 24): a lane holds two adjacent chunks and takes its elements'
+// partners from the LDS. 8192 tokens, 32/8 heads of 80 of which 20 turn, normed 52 us, rotary_any_kernel 140.
 template <typename T, int LPH>
 __global__ __launch_bounds__(256) void rotary_ragged_kernel(RotaryParams p, int32_t head_rows) {
   using E = Elem<T>;

@@ -1,14 +1,14 @@
 // Decode of rows whose leading keys lie in the same pages (a system prompt, a document, samples of one prompt): the
 // shared keys attended once for all rows, each row's own keys by itself, joined by log-sum-exp.
 //
-// A query that sees keys 0 .. L - 1, the first P of them shared, has o = sum_j e^(s_j) v_j / sum_j e^(s_j). Cut into ranges
-// of keys with partial outputs o_i and log-sum-exps l_i it is sum_i e^(l_i - M) o_i / sum_i e^(l_i - M) for any M, so the
-// shared ranges can be walked with every row's queries together: their keys are read rows times less often than by
-// lv_paged_attention (math of TorchAttention.decode, lean_vllm/attention/torch_backend.py:93-103, row by row).
+// A query that sees keys 0 .. L - 1, the first P of them shared, has o = sum_j e^(s_j) v_j / sum_j e^(s_j). Cut into
+// ranges of keys with partial outputs o_i and log-sum-exps l_i it is sum_i e^(l_i - M) o_i / sum_i e^(l_i - M) for any
+// M, so the shared ranges can be walked with every row's queries together: their keys are read rows times less often
+// than by lv_paged_attention (math of TorchAttention.decode, lean_vllm/attention/torch_backend.py:93-103, row by row).
 //
-// Two launches: the items, which are the prefix's (query tiles x kv heads x pieces of its keys) and the rows' own (rows x
-// kv heads x splits of their keys), and the merge of their fp32 partials. Everything is sized by the host from shapes and
-// bounds; the rows' lengths are read on the device, so a call can be captured.
+// Two launches: the items, which are the prefix's (query tiles x kv heads x pieces of its keys) and the rows' own
+// (rows x kv heads x splits of their keys), and the merge of their fp32 partials. Everything is sized by the host from
+// shapes and bounds; the rows' lengths are read on the device, so a call can be captured.
 //
 // What bounds it: the prefix's items MFMA once some 100 query rows share a kv head, the rows' own and small batches HBM.
 // The two kinds run in one launch, the prefix's first, on a grid that gives them one of the two workgroups that a CU holds
@@ -20,20 +20,20 @@
 //   2048, 128 rows, 64-1024, 16 a page    63.8            80.4                             149
 //   65,536, 256 rows, 16-64               287             312                              5786
 //   16,384, 16 rows, 64-512               24.9            38.6                             123
-// What is left at 200 rows: the prefix alone takes 134 us on whole CUs and 179 on one workgroup of each, the own keys alone
-// 161 (4 to 9 pieces of the prefix 231 / 240 / 252 / 264 / - / 281 us; raised wave priority of either kind 232 and 269;
-// partials stored past the caches 231; a last tile's empty waves that skip the products 232).
+// What is left at 200 rows: the prefix alone takes 134 us on whole CUs and 179 on one workgroup of each, the own keys
+// alone 161 (4 to 9 pieces of the prefix 231 / 240 / 252 / 264 / - / 281 us; raised wave priority of either kind 232
+// and 269; partials stored past the caches 231; a last tile's empty waves that skip the products 232).
 #include "few_item.h"
 
 namespace lv {
 
 constexpr int kSharedRound = 512;      // workgroups that run at once (two per CU)
-constexpr int kSharedPieceKeys = 256;  // and a piece of the prefix
+constexpr int kSharedPieceKeys = 256;  // least keys of a piece of the prefix
 constexpr int kMaxOwnSplits = 32;
 constexpr int kMaxSharedPieces = 256;
-// 64-key tiles of prompt items that the GPU takes in a microsecond with two workgroups on each CU (245; 190 with one); a
-// workgroup's time for a tile beside own items (1.3 alone on its CU); the rate at which own keys stream, and what their
-// items take besides. 32/8 heads of 128 and 64/8 of 64.
+// 64-key tiles of prompt items that the GPU takes in a microsecond with two workgroups on each CU (245; 190 with one);
+// a workgroup's time for a tile beside own items (1.3 alone on its CU); the rate at which own keys stream, and what
+// their items take besides. 32/8 heads of 128 and 64/8 of 64.
 constexpr double kTilesPerUs = 245, kTileUs = 2.0, kOwnBytesPerUs = 6.0e6, kOwnStartUs = 10;
 
 struct SharedParams : AttnParams {
@@ -43,8 +43,8 @@ struct SharedParams : AttnParams {
   int32_t splits, own_least;        // most splits of a row's own keys, and the least keys that one is cut for
 };
 
-// A row's own part: its keys from `start` on, in `n` splits of `per` (none where the row has no keys). A row that does not
-// see the whole prefix (its first query sees fewer keys) is attended by itself from key 0 on.
+// A row's own part: its keys from `start` on, in `n` splits of `per` (none where the row has no keys). A row that does
+// not see the whole prefix (its first query sees fewer keys) is attended by itself from key 0 on.
 struct OwnSpan {
   int start, per, n;
 };
@@ -61,9 +61,9 @@ __device__ __forceinline__ OwnSpan own_span(const SharedParams& p, int len) {
 // Partials lie by slot: piece i of token t's prefix in slot i tokens + t, its row's own split j in slot
 // (pieces + j) tokens + t.
 
-// How a kernel computes its items. Few<ROWS>: few-query items (few_item.h) of at most 16, 32 or 64 (query, head) rows, of
-// the prefix or of a row's own keys. Tile<TP>: prompt items (attn_common.h), 128 rows of the prefix against 64-key tiles
-// that the workgroup's waves share; TP: pages per 64-key tile, as there.
+// How a kernel computes its items. Few<ROWS>: few-query items (few_item.h) of at most 16, 32 or 64 (query, head) rows,
+// of the prefix or of a row's own keys. Tile<TP>: prompt items (attn_common.h), 128 rows of the prefix against 64-key
+// tiles that the workgroup's waves share; TP: pages per 64-key tile, as there.
 template <int ROWS, int HP = 1>
 struct Few {
   static constexpr int kRows = ROWS;
@@ -219,8 +219,8 @@ static SharedPlan shared_plan(int32_t rows, int32_t queries, int32_t hq, int32_t
   const int64_t tokens = (int64_t)rows * queries, query_rows = tokens * group;
   // Prompt items hold 128 rows; below, few-query items, which read no more than they need. 33 to 64 rows, few / prompt
   // items, prefixes of 2K, 16K, 64K: d128 17.9 / 15.0, 31.2 / 25.9, 74.5 / 67.8 us; d64 12.8 / -, 18.7 / 17.8, 36.5 /
-  // 35.9. 17 to 32 rows at d128 13.0 / 13.9, 23.4 / 23.3, 55.3 / 63.2. On pages that 64-key tiles do not fit, few-query
-  // items of 64 rows whatever their number.
+  // 35.9. 17 to 32 rows at d128 13.0 / 13.9, 23.4 / 23.3, 55.3 / 63.2. On pages that 64-key tiles do not fit,
+  // few-query items of 64 rows whatever their number.
   if (query_rows > (d == 64 ? 64 : 32))
     s.tile_pages = block_size % 64 == 0 ? 1 : block_size == 32 ? 2 : block_size == 16 ? 4 : 0;
   s.tile_rows = s.tile_pages > 0 ? kPrefillRows / group * group : few_rows(query_rows);
@@ -231,11 +231,11 @@ static SharedPlan shared_plan(int32_t rows, int32_t queries, int32_t hq, int32_t
   const double own_us = (double)own_keys * hkv * d * 4 / kOwnBytesPerUs;
   s.per_piece = kPrefillKeys;
   if (shared > 0) {
-    // Pieces: one workgroup of the prefix per CU beside the own keys (few-query items always: their prefix streams too, 64K
-    // keys for 2 rows 50.6 us against 52.5 with two), or two where the own keys are worth less than what half the
-    // workgroups lose (256 rows on 64K tokens 349 -> 288). And no more than make a piece end within the own keys' time:
-    // each costs its partials' way through memory (128 rows on 2K tokens, 1 / 2 / 4 / 8 pieces 78 / 65 / 68 / 74 us; 256
-    // on 1K, 1 / 2 / 4 / 8 68 / 74 / 78 / 85; 64 rows on 8K, 8 / 16 / 32 43 / 47 / 59).
+    // Pieces: one workgroup of the prefix per CU beside the own keys (few-query items always: their prefix streams
+    // too, 64K keys for 2 rows 50.6 us against 52.5 with two), or two where the own keys are worth less than what half
+    // the workgroups lose (256 rows on 64K tokens 349 -> 288). And no more than make a piece end within the own keys'
+    // time: each costs its partials' way through memory (128 rows on 2K tokens, 1 / 2 / 4 / 8 pieces 78 / 65 / 68 / 74
+    // us; 256 on 1K, 1 / 2 / 4 / 8 68 / 74 / 78 / 85; 64 rows on 8K, 8 / 16 / 32 43 / 47 / 59).
     const int64_t units = (int64_t)s.tiles * hkv, key_tiles = (shared + kPrefillKeys - 1) / kPrefillKeys;
     const bool beside = s.tile_pages == 0 || own_us > 0.3 * (double)(units * key_tiles) / kTilesPerUs;
     int64_t want = (beside ? kSharedRound / 2 : kSharedRound) / units;
@@ -245,11 +245,11 @@ static SharedPlan shared_plan(int32_t rows, int32_t queries, int32_t hq, int32_t
     s.per_piece = (int32_t)(((shared + want - 1) / want + 63) / 64 * 64);
     s.pieces = (shared + s.per_piece - 1) / s.per_piece;
   }
-  // Own keys: kv heads in pairs (512 adjacent bytes of a token) where those still make a workgroup for every second CU: 32
-  // rows on 8K tokens 39.3 -> 33.1 us, 4 rows of 8 kv heads 9.6 -> 11.4. Split to one round of the workgroups that the
-  // prefix leaves (64 rows on 8K: one split 49, two 43), or in two where there is more than a round (128 rows alone: one
-  // split 63.5, two 59.4, four 59.6), finer where rows are long. A split holds at least 384 keys where workgroups are
-  // many (256 rows on 1K 68.5 -> 67), 256 where they are few (4 rows 10.5 -> 9.7).
+  // Own keys: kv heads in pairs (512 adjacent bytes of a token) where those still make a workgroup for every second
+  // CU: 32 rows on 8K tokens 39.3 -> 33.1 us, 4 rows of 8 kv heads 9.6 -> 11.4. Split to one round of the workgroups
+  // that the prefix leaves (64 rows on 8K: one split 49, two 43), or in two where there is more than a round (128 rows
+  // alone: one split 63.5, two 59.4, four 59.6), finer where rows are long. A split holds at least 384 keys where
+  // workgroups are many (256 rows on 1K 68.5 -> 67), 256 where they are few (4 rows 10.5 -> 9.7).
   s.own_heads = hkv % 2 == 0 && (int64_t)rows * hkv >= kSharedRound / 2 && queries * group <= 16 ? 2 : 1;
   const int64_t units = (int64_t)rows * hkv / s.own_heads;
   const int64_t beside = std::max<int64_t>(kSharedRound - (int64_t)s.pieces * s.tiles * hkv, kSharedRound / 2);
@@ -335,8 +335,8 @@ extern "C" int lv_shared_prefix_decode(const void* q, int64_t q_stride_t, int64_
                                        int64_t table_stride, const int32_t* context_lens, int32_t num_rows,
                                        int32_t queries_per_row, int32_t num_heads, int32_t num_kv_heads,
                                        int32_t head_dim, float scale, int32_t shared_len, int32_t max_seqlen_k,
-                                       int64_t own_keys, void* out, int64_t out_stride_t, int64_t out_stride_h, void* workspace,
-                                       size_t workspace_bytes, int32_t dtype, void* stream) {
+                                       int64_t own_keys, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                                       void* workspace, size_t workspace_bytes, int32_t dtype, void* stream) {
   LV_REQUIRE(dtype == LV_DTYPE_BF16 || dtype == LV_DTYPE_F16, "shared_prefix_decode: dtype %d is not bf16 or fp16",
              dtype);
   const int rc = check_shared(num_rows, queries_per_row, num_heads, num_kv_heads, head_dim, block_size, shared_len,
