@@ -15,10 +15,10 @@
 // and the rows' own the other, so that one kind's MFMA work runs under the other's loads. Measured, 32/8 heads, d128, bf16
 // (prefix keys, rows, own keys a row; us):
 //                                         one launch      prefix, own and merge launches   lv_paged_attention
-//   32,768, 200 rows, 64-2048             231             303                              2380
-//   8192, 64 rows, 16-1024                43.1            60.8                             244
-//   2048, 128 rows, 64-1024, 16 a page    63.8            80.4                             149
-//   65,536, 256 rows, 16-64               287             312                              5786
+//   32,768, 200 rows, 64-2048             227             303                              2380
+//   8192, 64 rows, 16-1024                42.6            60.8                             244
+//   2048, 128 rows, 64-1024, 16 a page    61.1            80.4                             149
+//   65,536, 256 rows, 16-64               283             312                              5786
 //   16,384, 16 rows, 64-512               24.9            38.6                             123
 // What is left at 200 rows: the prefix alone takes 134 us on whole CUs and 179 on one workgroup of each, the own keys
 // alone 161 (4 to 9 pieces of the prefix 231 / 240 / 252 / 264 / - / 281 us; raised wave priority of either kind 232
@@ -139,26 +139,31 @@ __global__ __launch_bounds__(256, 2) void shared_items_kernel(SharedParams p, in
   Few<OWN_ROWS, HP>::template attend<T, D>(p, kvh, smem, part);
 }
 
-// One workgroup per (token, head): D / 4 threads a partial, 256 / (D / 4) partials at a time, joined through LDS.
-template <typename T, int D>
+// The merge of one (token, head)'s partials: D / 4 threads a partial, G partials at a time and BATCH such rounds' loads
+// in flight, the G threads of each four dims joined through LDS. A workgroup holds 256 / (D / 4) / G of them: few
+// partials each would leave most of a workgroup idle, and thousands of workgroups are three microseconds of launching
+// (6400 of 6 partials 11.2 -> 6.6 us, 256 rows on 1K shared tokens 67 -> 61.6 in all).
+constexpr int kMergeBatch = 8;
+template <typename T, int D, int G, int BATCH>
 __global__ __launch_bounds__(256) void shared_merge_kernel(SharedParams p) {
   using E = Elem<T>;
-  constexpr int LPR = D / 4, GROUPS = 256 / LPR, BATCH = 4;
-  __shared__ float part[GROUPS][D + 2];
-  const int tok = blockIdx.x / p.hq, head = blockIdx.x - tok * p.hq;
-  const int g = threadIdx.x / LPR, d0 = threadIdx.x % LPR * 4;
-  const int len = sload(p.lens_k + tok / p.queries);
-  const OwnSpan s = own_span(p, len);
+  constexpr int LPR = D / 4, PER = 256 / LPR / G;
+  __shared__ __attribute__((aligned(16))) float part[G > 1 ? PER * G : 1][D + 4];
+  const int slot = threadIdx.x / LPR, g = PER > 1 ? slot % G : slot, d0 = threadIdx.x % LPR * 4;
+  const int row = PER > 1 ? blockIdx.x * PER + slot / G : blockIdx.x;  // of the tokens x heads
+  const bool live = PER == 1 || row < p.tokens * p.hq;
+  const int tok = live ? row / p.hq : 0, head = live ? row - tok * p.hq : 0;
+  const OwnSpan s = own_span(p, p.lens_k[tok / p.queries]);
   const int shared = s.start > 0 ? p.pieces : 0;  // the partials: so many of the prefix, then s.n
-  const int count = shared + s.n;
+  const int count = live ? shared + s.n : 0;
   float m = -INFINITY, den = 0.f;
   f32x4 o = {0, 0, 0, 0};
-  for (int e0 = g; e0 < count; e0 += GROUPS * BATCH) {
+  for (int e0 = g; e0 < count; e0 += G * BATCH) {
     float ls[BATCH];
     f32x4 x[BATCH];
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
-      const int e = e0 + i * GROUPS;
+      const int e = e0 + i * G;
       ls[i] = -INFINITY;
       x[i] = f32x4{0, 0, 0, 0};
       if (e < count) {
@@ -181,25 +186,35 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedParams p) {
     }
     m = bm;
   }
-  *reinterpret_cast<f32x4*>(&part[g][d0]) = o;
-  if (d0 == 0) part[g][D] = m, part[g][D + 1] = den;
-  __syncthreads();
-  if (g > 0) return;
-  float bm = -INFINITY;
+  if constexpr (G > 1) {
+    *reinterpret_cast<f32x4*>(&part[slot][d0]) = o;
+    if (d0 == 0) part[slot][D] = m, part[slot][D + 1] = den;
+    __syncthreads();
+    if (g > 0) return;
+    float bm = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < GROUPS; ++i) bm = fmaxf(bm, part[i][D]);
-  const float base = merge_base(bm);
-  den = 0.f;
-  o = f32x4{0, 0, 0, 0};
+    for (int i = 0; i < G; ++i) bm = fmaxf(bm, part[slot + i][D]);
+    const float base = merge_base(bm);
+    den = 0.f;
+    o = f32x4{0, 0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < GROUPS; ++i) {
-    const float w = fast_exp2(part[i][D] - base);
-    den += w * part[i][D + 1];
-    o += w * *reinterpret_cast<const f32x4*>(&part[i][d0]);
+    for (int i = 0; i < G; ++i) {
+      const float w = fast_exp2(part[slot + i][D] - base);
+      den += w * part[slot + i][D + 1];
+      o += w * *reinterpret_cast<const f32x4*>(&part[slot + i][d0]);
+    }
   }
+  if (!live) return;
   o *= inv_sum(den);
   *reinterpret_cast<u32x2*>(p.out + (int64_t)tok * p.o_st + (int64_t)head * p.o_sh + d0 * 2) =
       u32x2{E::pack(o[0], o[1]), E::pack(o[2], o[3])};
+}
+
+template <typename T, int D, int G, int BATCH>
+static void launch_merge(const SharedParams& p, hipStream_t stream) {
+  constexpr int per = 256 / (D / 4) / G;
+  const int64_t rows = (int64_t)p.tokens * p.hq;
+  hipLaunchKernelGGL((shared_merge_kernel<T, D, G, BATCH>), dim3((uint32_t)((rows + per - 1) / per)), dim3(256), 0, stream, p);
 }
 
 // What the host decides from the shapes.
@@ -286,7 +301,11 @@ static int launch_shared(const SharedParams& p, const SharedPlan& s, hipStream_t
   else if (p.tile_rows == 32) launch_items<T, D, Few<32>>(p, s.own_heads, stream);
   else launch_items<T, D, Few<64>>(p, s.own_heads, stream);
   LV_LAUNCH_CHECK("shared_items_kernel");
-  hipLaunchKernelGGL((shared_merge_kernel<T, D>), dim3(p.tokens * p.hq), dim3(256), 0, stream, p);
+  // One batch of loads a thread where there are that many threads; all of a workgroup's where there are few rows.
+  const int most = p.pieces + p.splits;
+  if (most > 2 * kMergeBatch || (int64_t)p.tokens * p.hq < kSharedRound) launch_merge<T, D, 256 / (D / 4), 4>(p, stream);
+  else if (most > kMergeBatch) launch_merge<T, D, 2, kMergeBatch>(p, stream);
+  else launch_merge<T, D, 1, kMergeBatch>(p, stream);
   LV_LAUNCH_CHECK("shared_merge_kernel");
   return LV_OK;
 }

@@ -142,6 +142,15 @@ def test_every_kernel(cuda, name, dtype, dim):
     close(attend(cuda, 576, *s, dim ** -0.5), *want(*s, queries, dim ** -0.5))
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shared", [576, 2560, 6400])
+def test_every_merge(cuda, shared, dtype, dim):
+    """Some three, a dozen and two dozen partials a head of 40 rows (one, two or all of a workgroup's threads a head)."""
+    s = step(shared, [1 + i % 9 for i in range(40)], hq=16, hk=8, dim=dim, page=64, dtype=dtype, seed=shared)
+    close(attend(cuda, shared, *s, dim ** -0.5), *want(*s, 1, dim ** -0.5))
+
+
 @pytest.mark.parametrize("dim,page,rows", [(128, 16, 5), (64, 256, 5), (128, 48, 5), (128, 64, 70)])
 def test_rows_that_do_not_see_the_prefix(cuda, dim, page, rows):
     """Padding rows get zeros; a row shorter than the shared keys is attended by itself through its own table, whatever
