@@ -172,8 +172,8 @@ class MI355XAttention(AttentionBackend):
         out, o_args = output_heads(what, "out", q, out, like)
         if checks.ENABLED:
             checks.check_slots(slot_mapping, shape[0], shape[1])
-        _capi.call_on(device, "lv_append_kvcache", *q_args, *k_args, *v_args, pos, tab, held, width, interleaved, qw, kw,
-                      eps, tokens, heads, kv_heads, dim, *o_args, k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1],
+        _capi.call_on(device, "lv_append_kvcache", *q_args, *k_args, *v_args, pos, tab, held, width, int(interleaved), qw,
+                      kw, eps, tokens, heads, kv_heads, dim, *o_args, k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1],
                       cs[2], shape[1], slot_mapping.data_ptr(), _capi.DTYPES[dtype])
         return out
 
@@ -338,7 +338,6 @@ class MI355XAttention(AttentionBackend):
         kv_heads, dtype, device, qs = self.num_kv_heads, q.dtype, q.get_device(), q.stride()
         shape, cs = k_cache.shape, k_cache.stride()
         rows, width = bt.shape
-        page = shape[1]
         if dtype not in _capi.DTYPES or heads != self.num_heads or dim != self.head_dim or qs[2] != 1:
             raise ValueError(f"{what}: q is {dtype} {tuple(q.shape)} of strides {qs}, not bf16 or fp16 "
                              f"[T, {self.num_heads}, {self.head_dim}] of unit dim stride")
@@ -347,6 +346,7 @@ class MI355XAttention(AttentionBackend):
             raise ValueError(f"{what}: caches {tuple(shape)} and {tuple(v_cache.shape)} of {k_cache.dtype}, "
                              f"{v_cache.dtype}, strides {cs}, {v_cache.stride()}, for {kv_heads} kv heads of {dim} in "
                              f"{dtype}")
+        page = shape[1]
         if bt.dtype is not torch.int32 or lens.shape != (rows,) or (width > 1 and bt.stride(1) != 1):
             raise ValueError(f"{what}: block tables {bt.dtype} {tuple(bt.shape)} for {lens.numel()} rows")
         if rows == 0 or tokens % rows:
@@ -376,7 +376,7 @@ class MI355XAttention(AttentionBackend):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         _capi.call_on(device, "lv_shared_prefix_decode", q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(),
                       v_cache.data_ptr(), cs[0], cs[1], cs[2], page, bt.data_ptr(), bt.stride(0), lens.data_ptr(), *sizes,
-                      self.scale, shared_len, max_k, own_keys, out.data_ptr(), os_[0], os_[1], ws.data_ptr(), nbytes,
+                      float(self.scale), shared_len, max_k, own_keys, out.data_ptr(), os_[0], os_[1], ws.data_ptr(), nbytes,
                       _capi.DTYPES[dtype])
         return out
 

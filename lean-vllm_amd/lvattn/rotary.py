@@ -196,6 +196,6 @@ def _rotate(what, q, k, q_weight, k_weight, positions, table, eps, interleaved, 
     pos, tab, positions_held, width, qw, kw = rotary_args(what, positions, table, q_weight, k_weight, *like)
     out_q, oq_args = output_heads(what, "out_q", q, out_q, like)
     out_k, ok_args = output_heads(what, "out_k", k, out_k, like)
-    _capi.call_on(device, "lv_rotary", *q_args, *k_args, pos, tab, positions_held, width, interleaved, qw, kw, eps, tokens,
-                  heads, kv_heads, dim, *oq_args, *ok_args, _capi.DTYPES[dtype])
+    _capi.call_on(device, "lv_rotary", *q_args, *k_args, pos, tab, positions_held, width, int(interleaved), qw, kw, eps,
+                  tokens, heads, kv_heads, dim, *oq_args, *ok_args, _capi.DTYPES[dtype])
     return out_q, out_k

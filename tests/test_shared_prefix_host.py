@@ -40,7 +40,7 @@ def args(q=(4, 8, 64), cache=(10, 16, 2, 64), tables=(4, 6), lens=4, dtype=BF, c
 
 @pytest.mark.parametrize("change,message", [
     (dict(dtype=torch.float32), "not bf16 or fp16"), (dict(q=(4, 6, 64)), "q is"), (dict(q=(4, 8, 128)), "q is"),
-    (dict(cache=(10, 16, 4, 64)), "caches"), (dict(cache_dtype=torch.float16), "caches"),
+    (dict(cache=(10, 16, 4, 64)), "caches"), (dict(cache=(64,)), "caches"), (dict(cache_dtype=torch.float16), "caches"),
     (dict(q=(5, 8, 64)), "do not divide"), (dict(lens=0, tables=(0, 6)), "do not divide"),
     (dict(tables=(3, 6)), "block tables"), (dict(table_dtype=torch.int64), "block tables"),
     (dict(tables=(4, 1)), "32 shared keys are not whole pages of 16 within tables of 1"), (dict(), "on one GPU"),
