@@ -178,12 +178,60 @@ PyObject* count_ids(PyObject*, PyObject* lists) {
   return PyLong_FromSsize_t(total);
 }
 
+// common_blocks(block_lists) -> how many block ids all the lists begin with alike: each row against the first, as far as
+// the rows before agreed.
+PyObject* common_blocks(PyObject*, PyObject* lists) {
+  PyObject *h = nullptr, *h0 = nullptr;
+  PyObject **il, **first;
+  Py_ssize_t rows, n = 0;
+  long* ids = nullptr;
+  PyObject* result = nullptr;
+  if (!items_of(lists, &il, &rows, &h)) return nullptr;
+  if (rows > 0) {
+    if (!items_of(il[0], &first, &n, &h0)) goto done;
+    ids = static_cast<long*>(PyMem_Malloc(sizeof(long) * (n > 0 ? n : 1)));
+    if (!ids) {
+      PyErr_NoMemory();
+      goto done;
+    }
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      ids[i] = PyLong_AsLong(first[i]);
+      if (ids[i] == -1 && PyErr_Occurred()) goto done;
+    }
+  }
+  for (Py_ssize_t r = 1; r < rows && n > 0; ++r) {
+    PyObject* hr = nullptr;
+    PyObject** row;
+    Py_ssize_t len, i = 0;
+    if (!items_of(il[r], &row, &len, &hr)) goto done;
+    if (len < n) n = len;
+    for (; i < n; ++i) {
+      if (row[i] == first[i]) continue;  // the same int object, as rows of one prefix cache often hold
+      const long id = PyLong_AsLong(row[i]);
+      if (id == -1 && PyErr_Occurred()) {
+        Py_DECREF(hr);
+        goto done;
+      }
+      if (id != ids[i]) break;
+    }
+    n = i;
+    Py_DECREF(hr);
+  }
+  result = PyLong_FromSsize_t(n);
+done:
+  PyMem_Free(ids);
+  Py_XDECREF(h0);
+  Py_DECREF(h);
+  return result;
+}
+
 PyMethodDef methods[] = {
     {"stage_rows", stage_rows, METH_VARARGS,
      "stage_rows(num_cached, num_new, block_lists, address, capacity) -> (rows, n_ids, width)"},
     {"stage_graph_rows", stage_graph_rows, METH_VARARGS,
      "stage_graph_rows(num_cached, block_lists, address, capacity, bs, q) -> (rows, n_ids, width)"},
     {"count_ids", count_ids, METH_O, "count_ids(block_lists) -> total block ids"},
+    {"common_blocks", common_blocks, METH_O, "common_blocks(block_lists) -> block ids that all lists begin with alike"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hoststage", "Host staging of the packing inputs.", -1, methods};

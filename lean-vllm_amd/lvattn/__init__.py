@@ -15,9 +15,8 @@
 from .abstract import AttentionBackend, LayerSpec, write_into
 from .backend import MI355XAttention
 from .merge import merge_attention, merge_attention_
-from .context import (Context, get_context, reset_context, set_context, shared_prefix_len, split_decodes_and_prefills,
-                      use_context)
-from .pack import Packer, StagingBuffers, decode_query_len
+from .context import Context, get_context, reset_context, set_context, split_decodes_and_prefills, use_context
+from .pack import Packer, StagingBuffers, decode_query_len, shared_prefix_len
 from .graphs import DecodeGraphs
 from .rotary import apply_rotary, norm_rotary, rotary_frequencies, rotary_table
 from .mla import whole_context

@@ -86,28 +86,6 @@ def split_decodes_and_prefills(context, query_len: int = 1):
     return cache[query_len]
 
 
-def shared_prefix_len(block_lists, num_cached, block_size: int) -> int:
-    """Keys that every row of a decode step finds in the same pages: the whole pages (``block_size`` keys each) that all
-    ``block_lists`` begin with, as far as every row's ``num_cached`` keys reach. 0 for a single row, which shares nothing.
-    For ``MI355XAttention.decode_shared``; rows and lists as ``Packer.pack`` takes them."""
-    if len(block_lists) != len(num_cached):
-        raise ValueError(f"shared_prefix_len: {len(block_lists)} block lists for {len(num_cached)} rows")
-    if len(block_lists) < 2:
-        return 0
-    most = min(int(min(num_cached)) // block_size, min(len(b) for b in block_lists))
-    first = block_lists[0]
-    # The shared pages lead: found by bisection, a slice compared per row and step.
-    lo, hi = 0, most
-    while lo < hi:
-        mid = (lo + hi + 1) // 2
-        head = list(first[lo:mid])
-        if all(list(b[lo:mid]) == head for b in block_lists):
-            lo = mid
-        else:
-            hi = mid - 1
-    return lo * block_size
-
-
 _CONTEXT = Context()
 
 

@@ -114,6 +114,17 @@ def check_block_lists(num_cached, num_new, lengths, block_size: int) -> None:
                          f"{int(num_cached[i])} + {int(num_new[i])} tokens need {int(need[i])}")
 
 
+def shared_prefix_len(block_lists, num_cached, block_size: int) -> int:
+    """Keys that every row of a decode step finds in the same pages: the whole pages (``block_size`` keys each) that all
+    ``block_lists`` begin with, as far as every row's ``num_cached`` keys reach. 0 for a single row, which shares nothing.
+    For ``MI355XAttention.decode_shared``; rows and lists as ``Packer.pack`` takes them, compared by ``_hoststage``."""
+    if len(block_lists) != len(num_cached):
+        raise ValueError(f"shared_prefix_len: {len(block_lists)} block lists for {len(num_cached)} rows")
+    if len(block_lists) < 2:
+        return 0
+    return min(int(min(num_cached)) // block_size, _host_stage().common_blocks(block_lists)) * block_size
+
+
 class Packer:
     """Builds a step's attention ``Context`` fields on the GPU from per-row scheduler state.
 

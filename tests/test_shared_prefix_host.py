@@ -1,5 +1,11 @@
 """decode_shared's host side on the CPU: the shared length, refusals of the Python call and of the C entry."""
 
+import shutil
+import subprocess
+import sys
+import sysconfig
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -26,6 +32,64 @@ def test_shared_prefix_len():
         assert shared_prefix_len([a, b, a], [12 * 8] * 3, 8) == 8 * n
     with pytest.raises(ValueError, match="2 block lists for 1 rows"):
         shared_prefix_len([head, head], [64], 16)
+
+
+def test_common_blocks_under_every_kind_of_row():
+    from lvattn import _hoststage as hs
+
+    assert hs.common_blocks([]) == 0 and hs.common_blocks([[]]) == 0 and hs.common_blocks([[5, 6]]) == 2
+    assert hs.common_blocks([(1, 2, 3), np.array([1, 2, 4]), [1, 2]]) == 2
+    assert hs.common_blocks([[1, 2], [], [1, 2]]) == 0
+    for bad in (3, [[1], 3], [["a"], [1]], [[1], ["a"]], [[1 << 70], [1]]):
+        with pytest.raises((TypeError, OverflowError)):
+            hs.common_blocks(bad)
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="no g++")
+def test_common_blocks_under_the_address_sanitizer(tmp_path):
+    """The program of test_host_asan.py, driving common_blocks over ragged lists of every kind."""
+    from test_host_asan import DRIVER, SOURCE
+
+    libdir, ldver = sysconfig.get_config_var("LIBDIR"), sysconfig.get_config_var("LDVERSION")
+    if not (Path(libdir) / f"libpython{ldver}.so").exists():
+        pytest.skip("no shared libpython to embed")
+    (tmp_path / "driver.cpp").write_text(DRIVER)
+    (tmp_path / "script.py").write_text(SCRIPT)
+    exe = tmp_path / "common"
+    build = subprocess.run(
+        ["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", f"-I{sysconfig.get_paths()['include']}",
+         str(SOURCE), str(tmp_path / "driver.cpp"), f"-L{libdir}", f"-lpython{ldver}", f"-Wl,-rpath,{libdir}", "-o",
+         str(exe)], capture_output=True, text=True)
+    assert build.returncode == 0, build.stderr[-3000:]
+    env = {"ASAN_OPTIONS": "detect_leaks=0:halt_on_error=1", "UBSAN_OPTIONS": "halt_on_error=1",
+           "PYTHONHOME": sys.base_prefix, "PATH": "/usr/bin:/bin"}
+    run = subprocess.run([str(exe), str(tmp_path / "script.py")], capture_output=True, text=True, env=env, timeout=300)
+    assert run.returncode == 0 and "common ok" in run.stdout, run.stdout[-2000:] + run.stderr[-4000:]
+
+
+SCRIPT = """
+import random
+import _hoststage as hs
+import numpy as np
+rng = random.Random(0)
+for trial in range(2000):
+    head = [rng.randint(0, 1 << 31) for _ in range(rng.randint(0, 20))]
+    rows = []
+    for r in range(rng.randint(1, 8)):
+        ids = head[:rng.randint(0, len(head))] + [rng.randint(0, 3) for _ in range(rng.randint(0, 4))]
+        rows.append([list, tuple, lambda x: np.asarray(x, dtype=np.int64)][rng.randrange(3)](ids))
+    want = 0
+    while all(len(x) > want for x in rows) and len({int(x[want]) for x in rows}) == 1:
+        want += 1
+    assert hs.common_blocks(rows) == want, (rows, want)
+    assert hs.common_blocks(tuple(rows)) == want
+    try:
+        hs.common_blocks(rows[:1] + [7] + rows)
+        assert len(rows[0]) == 0
+    except TypeError:
+        pass
+print("common ok")
+"""
 
 
 BF = torch.bfloat16
