@@ -241,7 +241,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int32_t hea
 
 // The same rows with a rotary width that is no multiple of 16 (interleaved: 8), so that a pair's elements lie in other
 // lanes (quarters of 80- and 96-wide heads: 20 and 24): a lane holds two adjacent chunks and takes its elements'
-// partners from the LDS. 8192 tokens, 32/8 heads of 80 of which 20 turn, normed 52 us, rotary_any_kernel 140.
+// partners, and the table's row, from the LDS. 8192 tokens, 32/8 heads of 80 of which 20 turn, normed, us: 45; the table
+// read from memory by each lane 52; the partners too 79; rotary_any_kernel 140.
 template <typename T, int LPH>
 __global__ __launch_bounds__(256) void rotary_ragged_kernel(RotaryParams p, int32_t head_rows) {
   using E = Elem<T>;
@@ -254,6 +255,12 @@ __global__ __launch_bounds__(256) void rotary_ragged_kernel(RotaryParams p, int3
   HeadRow row = head_row(p, t, min(h, head_rows - 1));
   if (h >= head_rows || !holds) row.dst = nullptr;
   u32x4 x[2] = {ld16(row.src + 2 * d0), ld16(row.src + 2 * d0 + 16)};
+  // The token's table row, once for the wave's head rows (p.rot <= p.dim <= 256).
+  __shared__ float turns[4][256];
+  float* turn = turns[threadIdx.x >> 6];
+  float amp;
+  const float* row_table = table_row(p, p.positions[t], amp);
+  for (int i = lane; i < p.rot; i += 64) turn[i] = row_table[i] * amp;
   float e[16];
 #pragma unroll
   for (int i = 0; i < 8; ++i) e[2 * i] = E::lo(x[i / 4][i % 4]), e[2 * i + 1] = E::hi(x[i / 4][i % 4]);
@@ -282,8 +289,6 @@ __global__ __launch_bounds__(256) void rotary_ragged_kernel(RotaryParams p, int3
   for (int i = 0; i < 16; ++i) mine[17 * (lane % LPH) + i] = e[i];
   __builtin_amdgcn_wave_barrier();
   if (row.turned && d0 < p.rot) {
-    float amp;
-    const float* row_table = table_row(p, p.positions[t], amp);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int d = min(d0 + i, p.rot - 1);
@@ -291,7 +296,7 @@ __global__ __launch_bounds__(256) void rotary_ragged_kernel(RotaryParams p, int3
       const int pair = p.interleaved ? d / 2 : second ? d - half : d;
       const int other = p.interleaved ? d ^ 1 : second ? pair : d + half;
       const float y = mine[other + other / 16];
-      const float c = row_table[pair] * amp, s = row_table[half + pair] * amp;
+      const float c = turn[pair], s = turn[half + pair];
       if (d0 + i < p.rot) e[i] = second ? e[i] * c + y * s : e[i] * c - y * s;
     }
   }
